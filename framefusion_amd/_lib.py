@@ -108,6 +108,43 @@ class FFLqArgs(C.Structure):
 LQ_ARGS = struct.Struct("=2Q7qdq3Q")
 
 
+class FFRotary(C.Structure):
+    """ff_rotary_t (every member 8 bytes wide: ROTARY.pack)."""
+    _fields_ = ([(f, C.c_void_p) for f in ("q", "k", "q_out", "k_out", "cos", "sin")]
+                + [(f, C.c_int64) for f in ("dtype", "table_dtype", "B", "L", "H", "H_kv", "dh", "rot", "q_batch", "q_head", "q_token", "k_batch",
+                                            "k_head", "k_token", "qo_batch", "qo_head", "qo_token", "ko_batch", "ko_head", "ko_token", "t_axis",
+                                            "t_batch", "t_token", "sec0", "sec1", "interleaved", "transpose")]
+                + [("stream", C.c_void_p)])
+
+
+ROTARY = struct.Struct("=6Q27qQ")
+
+
+class FFCache(C.Structure):
+    """ff_cache_t (CACHE, the head of the three structures below)."""
+    _fields_ = ([(f, C.c_void_p) for f in ("keys", "values", "key_scales", "value_scales", "table", "start")]
+                + [(f, C.c_int64) for f in ("store", "n_pages", "kv_heads", "page_size", "dh", "table_width", "B", "n", "dtype")])
+
+
+class FFCacheRows(C.Structure):
+    """ff_cache_rows_t (CACHE_ROWS)."""
+    _fields_ = ([("cache", FFCache), ("k", C.c_void_p), ("v", C.c_void_p)]
+                + [(f, C.c_int64) for f in ("k_batch", "k_head", "k_token", "v_batch", "v_head", "v_token")] + [("stream", C.c_void_p)])
+
+
+class FFCacheAttention(C.Structure):
+    """ff_cache_attention_t (CACHE_ATTENTION)."""
+    _fields_ = ([("cache", FFCache), ("q", C.c_void_p), ("out", C.c_void_p), ("mask", C.c_void_p), ("ws", C.c_void_p), ("ws_bytes", C.c_size_t)]
+                + [(f, C.c_int64) for f in ("H", "q_batch", "q_head", "q_token", "o_batch", "o_head", "o_token", "mask_batch")]
+                + [("scale", C.c_double), ("stream", C.c_void_p)])
+
+
+CACHE = struct.Struct("=6Q9q")
+CACHE_ROWS = struct.Struct("=6Q9q2Q6qQ")
+CACHE_ATTENTION = struct.Struct("=6Q9q5Q8qdQ")
+STORE_E2M1, STORE_E4M3 = 4, 8
+
+
 class FFSegment(C.Structure):
     _fields_ = [("begin", C.c_int32), ("count", C.c_int32), ("first", C.c_int32), ("period", C.c_int32)]
 
@@ -156,6 +193,13 @@ PROTOTYPES = {
     "ff_host_free": (None, [_vp]),
     "ff_ctx_last_query_importance": (_i32, [_vp, _vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f64, _i32, _vp, _vp, _i64, _i64,
                                             _i64, _vp, _sz, _vp]),
+    "ff_rotary_tables": (_i32, [_vp, _i64, _vp, _i64, _f64, _i32, _i32, _vp, _vp, _vp]),
+    "ff_rotary_apply": (_i32, [_vp]),
+    "ff_cache_write": (_i32, [_vp]),
+    "ff_cache_read": (_i32, [_vp]),
+    "ff_cache_keep": (_i32, [_vp, _vp, _i64, _vp]),
+    "ff_cache_attention_workspace_bytes": (_sz, [_vp]),
+    "ff_cache_attention": (_i32, [_vp]),
     "ff_merge_step": (_i32, [_vp, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _i64, _i32, _f64, _f64, _f64, _vp, _vp, _vp, _vp,
                              _vp, _vp, _vp, _vp, _i64, C.POINTER(FFAux), _i32, _i64, _i64, _vp, _vp, _vp, _sz, _vp]),
 }
@@ -261,7 +305,8 @@ def load():
     got = lib.ff_abi_version()
     if got != ABI_VERSION:
         raise FrameFusionHipError(f"ABI mismatch: library {got}, binding {ABI_VERSION}")
-    for which, cls in enumerate((FFCtx, FFMergeCall, FFMergeResult, FFPruneCall, FFAux, FFLqArgs)):
+    for which, cls in enumerate((FFCtx, FFMergeCall, FFMergeResult, FFPruneCall, FFAux, FFLqArgs, FFRotary, FFCache, FFCacheRows,
+                                 FFCacheAttention)):
         if lib.ff_abi_sizeof(which) != C.sizeof(cls):
             raise FrameFusionHipError(f"ABI mismatch: sizeof({cls.__name__}) is {C.sizeof(cls)} here, "
                                       f"{lib.ff_abi_sizeof(which)} in the library")

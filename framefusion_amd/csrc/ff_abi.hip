@@ -257,6 +257,10 @@ extern "C" size_t ff_abi_sizeof(int which) {
         case 3: return sizeof(ff_prune_call_t);
         case 4: return sizeof(ff_aux_t);
         case 5: return sizeof(ff_lq_args_t);
+        case 6: return sizeof(ff_rotary_t);
+        case 7: return sizeof(ff_cache_t);
+        case 8: return sizeof(ff_cache_rows_t);
+        case 9: return sizeof(ff_cache_attention_t);
         default: return 0;
     }
 }

@@ -374,8 +374,92 @@ int ff_ctx_reset(ff_ctx_t* ctx, ff_stream_t stream);
 void* ff_host_alloc(size_t bytes);
 void ff_host_free(void* p);
 
+/* ---- decoding behind a reduced prefill: rotary positions, a paged (quantised) cache, attention of new tokens over it ----
+ * All strides are in ELEMENTS of the tensor's type; a head's `dh` channels are contiguous; T = FF_F32 / FF_BF16 / FF_F16.
+ *
+ * ff_rotary_tables: position tables in the layout a decoder stack threads through its layers.  For each of the n positions
+ *   a_i = position * inv_freq[i] (formed and reduced in 64 bits), cos = T(factor * cos a), sin = T(factor * sin a), rows of
+ *   2 * half: [a, a] (half layout) or a_i at 2i and 2i + 1 (interleaved).
+ * ff_rotary_apply: y = x rotated by the tables, fp32 inside, one rounding.  Half layout: pair (i, i + rot/2), interleaved: pair
+ *   (2i, 2i + 1); y1 = x1 c1 - x2 s1, y2 = x2 c2 + x1 s2 (transpose != 0, the gradient: y1 = x1 c1 + x2 s2, y2 = x2 c2 - x1 s1).
+ *   Channels >= rot are copied.  sec0 + sec1 > 0 (half layout): pair i takes its table row from axis 0 for i < sec0, axis 1 for
+ *   i < sec0 + sec1, else axis 2 (M-RoPE).  16-byte accesses when rows, strides and rot allow, else one element at a time. */
+typedef struct ff_rotary {
+    const void* q;               /* [B, H, L, dh]                                                        */
+    const void* k;               /* [B, H_kv, L, dh] or NULL with H_kv = 0                               */
+    void* q_out;
+    void* k_out;
+    const void* cos;             /* [axes, B or 1, L, rot]                                               */
+    const void* sin;
+    int64_t dtype, table_dtype, B, L, H, H_kv, dh, rot;
+    int64_t q_batch, q_head, q_token, k_batch, k_head, k_token;          /* strides of the inputs ...    */
+    int64_t qo_batch, qo_head, qo_token, ko_batch, ko_head, ko_token;    /* ... and of the outputs       */
+    int64_t t_axis, t_batch, t_token;                                    /* strides of both tables       */
+    int64_t sec0, sec1, interleaved, transpose;
+    ff_stream_t stream;
+} ff_rotary_t;
+int ff_rotary_tables(const int64_t* positions, int64_t n, const double* inv_freq, int64_t half, double factor, int interleaved,
+                     int dtype, void* cos, void* sin, ff_stream_t stream);
+int ff_rotary_apply(const ff_rotary_t* args);
+
+/* The cache: keys and values [n_pages, kv_heads, page_size, dh] in T (store = the dtype code) or as codes with one scale byte
+ * for each 32 channels, [n_pages, kv_heads, page_size, dh / 32]: value = code * 2^(byte - 127), byte 0 = the block is zero, 255 = it is NaN.
+ * FF_STORE_E4M3: one byte a channel.  FF_STORE_E2M1: half a byte, the even channel in the low half.  Position p of sequence b
+ * is row p % page_size of page table[b * table_width + p / page_size]; a position past the table or with an entry outside
+ * [0, n_pages) has no place: it is not written, reads as zeros and is not attended to.  start[b] = tokens before the n that
+ * the call is about; start[b] < 0 marks a padding row (nothing written, zeros out).  page_size: multiple of 16; dh: multiple
+ * of 32 up to 256 (attention: 32, 64, 128 or 256); a table covers at most 2^31 - 2^16 positions.
+ *
+ * ff_cache_write: n tokens from start[b] on.  Block scale 2^e: the smallest e with max|x| <= 448 * 2^e (e4m3) or 6 * 2^e (e2m1),
+ *   e >= -100; codes round to nearest even.  |x| is first limited to 1.875 (e4m3) / 1.5 (e2m1) * 2^127 (FF_F16: 2^15), so that every
+ *   stored value is finite in T; a block with a NaN or infinity is stored as NaN.
+ * ff_cache_read: the values of n tokens from start[b] on, rounded once to T.
+ * ff_cache_keep: row start[b] + i becomes a copy of row start[b] + accepted[b * m + i]; the list ends at the first entry that
+ *   is negative, not larger than the one before, or without a place. */
+enum { FF_STORE_E2M1 = 4, FF_STORE_E4M3 = 8 };
+typedef struct ff_cache {
+    void* keys;
+    void* values;
+    uint8_t* key_scales;         /* NULL for a store in T                                                */
+    uint8_t* value_scales;
+    const int32_t* table;        /* [B, table_width]                                                     */
+    const int32_t* start;        /* [B]                                                                  */
+    int64_t store, n_pages, kv_heads, page_size, dh, table_width, B, n, dtype;
+} ff_cache_t;
+typedef struct ff_cache_rows {
+    ff_cache_t cache;
+    void* k;                     /* [B, kv_heads, n, dh] of T: read by write, written by read            */
+    void* v;
+    int64_t k_batch, k_head, k_token, v_batch, v_head, v_token;
+    ff_stream_t stream;
+} ff_cache_rows_t;
+int ff_cache_write(const ff_cache_rows_t* args);
+int ff_cache_read(const ff_cache_rows_t* args);
+int ff_cache_keep(const ff_cache_t* cache, const int32_t* accepted, int64_t m, ff_stream_t stream);
+
+/* ff_cache_attention: out_i = sum_j softmax_j(scale q_i . k_j) v_j for the n new tokens of each sequence, whose keys and values
+ *   lie in the cache behind its start[b] earlier ones.  Token i sees every earlier token, and new token j where
+ *   mask[b * mask_batch + i * n + j] != 0 (mask = NULL: j <= i).  What it does not see contributes nothing, whatever is stored
+ *   there; a token that sees nothing gets zeros.  Scores, statistics and sums in fp32; the probabilities are rounded to T before
+ *   they meet the values.  ws: ff_cache_attention_workspace_bytes(args) bytes (may be 0), not initialised, dead when the call's
+ *   work is done. */
+typedef struct ff_cache_attention {
+    ff_cache_t cache;
+    const void* q;               /* [B, H, n, dh]                                                        */
+    void* out;                   /* [B, H, n, dh]                                                        */
+    const uint8_t* mask;
+    void* ws;
+    size_t ws_bytes;
+    int64_t H, q_batch, q_head, q_token, o_batch, o_head, o_token, mask_batch;
+    double scale;
+    ff_stream_t stream;
+} ff_cache_attention_t;
+size_t ff_cache_attention_workspace_bytes(const ff_cache_attention_t* args);
+int ff_cache_attention(const ff_cache_attention_t* args);
+
 /* sizeof() of the structures above as THIS library was compiled (0: ff_ctx_t, 1: ff_merge_call_t, 2: ff_merge_result_t,
- * 3: ff_prune_call_t, 4: ff_aux_t, 5: ff_lq_args_t), so a binding can verify its own layout. */
+ * 3: ff_prune_call_t, 4: ff_aux_t, 5: ff_lq_args_t, 6: ff_rotary_t, 7: ff_cache_t, 8: ff_cache_rows_t, 9: ff_cache_attention_t),
+ * so a binding can verify its own layout. */
 size_t ff_abi_sizeof(int which);
 
 #ifdef __cplusplus
