@@ -1,58 +1,602 @@
 // ff_attend.hip - attention of the new tokens of each sequence (one, a chunk, or a tree of drafted ones) over the paged cache.
+//
+// All query rows that share a kv head - n tokens times G heads - are one matrix of R = n G rows, so the cache is read once for
+// all of them.  A wave works on 32 keys at a time, alone, with nothing in shared memory:
+//   S^T = K Q^T   keys are the rows of the first operand, channels its contraction.  A lane owns a key (lane & 15) and a quarter
+//                 of its channels (lane >> 4); WHICH channels is free as long as Q agrees, so they are whole 16-byte loads.
+//   softmax       S^T leaves a lane with 8 scores of ONE query row: maximum and sum need two cross-lane steps each.
+//   O^T = V^T P^T the second operand wants, in each lane, 8 keys of one query row - which is what the lane has.  The first wants
+//                 8 keys of one channel: a lane loads dh / 16 consecutive channels of each of its 8 keys and turns that block
+//                 over in registers (v_perm), the channels of a tile being every (dh / 16)-th one.
+// Codes become T by the scaled conversions of gfx950, one scale a block, exact (a code times a power of two fits T's mantissa).
+// The four waves of a workgroup take every fourth tile of 32 keys and are summed through shared memory; long caches are split over
+// workgroups, whose partial rows (maximum, sum, unscaled output, all fp32) a second launch joins in fixed order.
 #include "ff_cache.h"
 
 namespace ff {
 
-// One wave to a query row.  Lanes take keys for the scores (64 at a time, running maximum and sum in fp32), channels for the
-// values.
-template <int DT, int STORE>
-__global__ __launch_bounds__(64) void k_cache_attention(const ff_cache_attention_t a) {
-    __shared__ float s_q[256];
-    const ff_cache_t& c = a.cache;
-    const int lane = threadIdx.x, dh = (int)c.dh, kv = (int)c.kv_heads, n = (int)c.n;
-    const uint32_t h = blockIdx.y, b = blockIdx.x / (uint32_t)n, i = blockIdx.x - b * (uint32_t)n;
-    const int head = (int)(h / (uint32_t)(a.H / kv));
-    const int32_t* table = c.table + (int64_t)b * c.table_width;
-    const int64_t start = c.start[b];
-    char* out = (char*)a.out + ((int64_t)b * a.o_batch + h * a.o_head + i * a.o_token) * Act<DT>::kBytes;
-    for (int e = lane; e < dh; e += 64) s_q[e] = Act<DT>::load1(a.q, (int64_t)b * a.q_batch + h * a.q_head + i * a.q_token + e);
-    __syncthreads();
-    const int64_t end = start < 0 ? 0 : min(start + n, c.table_width * c.page_size);
-    float m = -__builtin_inff(), l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int64_t j0 = 0; j0 < end; j0 += 64) {
-        const int64_t j = j0 + lane;
-        const int64_t row = j < end ? cache_row(table, c.table_width, c.n_pages, (int)c.page_size, kv, head, j) : -1;
-        bool seen = row >= 0;
-        if (seen && j >= start) seen = a.mask ? a.mask[(int64_t)b * a.mask_batch + (int64_t)i * n + (j - start)] != 0 : j - start <= i;
-        float s = -__builtin_inff();
-        if (seen) {
-            s = 0.f;
-            for (int u = 0; u < dh / 8; ++u) {
-                float f[8];
-                fetch8<DT, STORE>(c.keys, c.key_scales, row, dh, u, f);
-                for (int e = 0; e < 8; ++e) s = fmaf(s_q[u * 8 + e], f[e], s);
-            }
-            s *= (float)a.scale;
-        }
-        float top = s;
-        for (int k = 32; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor(top, k, 64));
-        const float m_new = fmaxf(m, top), base = m_new == -__builtin_inff() ? 0.f : m_new;
-        const float down = __expf(m - base), p = seen ? __expf(s - base) : 0.f;
-        l = l * down + wave_sum(p);
-        m = m_new;
-        for (int k = 0; k < 4; ++k) o[k] *= down;
-        for (int k = 0; k < 64; ++k) {
-            const int64_t r = __shfl(row, k, 64);
-            const float w = __shfl(p, k, 64);
-            if (!__shfl((int)seen, k, 64)) continue;
-            if (lane * 4 >= dh) continue;
-            float f[8];
-            fetch8<DT, STORE>(c.values, c.value_scales, r, dh, lane / 2, f);
-            for (int e = 0; e < 4; ++e) o[e] = fmaf(w, f[(lane & 1) * 4 + e], o[e]);
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kAttWaves = 4;
+constexpr int kAttTile = 32;                       // keys of one step of a wave
+constexpr float kNone = -__builtin_inff();
+
+// ---- 8 elements of a lane in the operands of a product over 8 x 4 of them ------------------------------------------------
+template <int DT> struct Frag { uint32_t w[4]; };
+template <> struct Frag<FF_F32> { float w[8]; };
+
+template <int DT> __device__ inline f32x4 mma(const Frag<DT>& a, const Frag<DT>& b, f32x4 c) {
+    if constexpr (DT == FF_BF16) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    } else if constexpr (DT == FF_F16) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.w[e], b.w[e], c, 0, 0, 0);
+        return c;
+    }
+}
+
+template <int DT> __device__ inline uint32_t pack2(float a, float b) {      // two floats rounded to T (16 bits)
+    if constexpr (DT == FF_BF16) {
+        bf16x2_t p;
+        p.x = (__bf16)a;
+        p.y = (__bf16)b;
+        return __builtin_bit_cast(uint32_t, p);
+    } else {
+        half2_t p;
+        p.x = (_Float16)a;
+        p.y = (_Float16)b;
+        return __builtin_bit_cast(uint32_t, p);
+    }
+}
+// two codes of a stored word as T: 8 bits - pair `i` of 2, 4 bits - pair `i` of 4
+template <int DT, int STORE> __device__ inline uint32_t codes2(uint32_t w, float scale, int i) {
+    if constexpr (STORE == FF_STORE_E4M3) {
+        if constexpr (DT == FF_BF16)
+            return i ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true))
+                     : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false));
+        else
+            return i ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, true))
+                     : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, false));
+    } else {
+        if constexpr (DT == FF_BF16) {
+            return i == 0 ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0))
+                 : i == 1 ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1))
+                 : i == 2 ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2))
+                          : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3));
+        } else {
+            return i == 0 ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 0))
+                 : i == 1 ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 1))
+                 : i == 2 ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 2))
+                          : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 3));
         }
     }
-    if (lane * 4 < dh)
-        for (int e = 0; e < 4; ++e) Act<DT>::store1(out, lane * 4 + e, l > 0.f || l != l ? o[e] / l : 0.f);
+}
+template <int STORE> __device__ inline f32x2 codes2_f32(uint32_t w, float scale, int i) {
+    f32x2 f;
+    if constexpr (STORE == FF_STORE_E4M3) {
+        f = i ? __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
+    } else {
+        f = i == 0 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0) : i == 1 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1)
+          : i == 2 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2) : __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3);
+    }
+    f.x *= scale;
+    f.y *= scale;
+    return f;
+}
+
+// N bytes (a power of two) from p into words
+template <int N> __device__ inline void load_words(const char* p, uint32_t* w) {
+    if constexpr (N == 1) {
+        w[0] = *(const uint8_t*)p;
+    } else if constexpr (N == 2) {
+        w[0] = *(const uint16_t*)p;
+    } else if constexpr (N == 4) {
+        w[0] = *(const uint32_t*)p;
+    } else if constexpr (N == 8) {
+        const uint2 v = *(const uint2*)p;
+        w[0] = v.x; w[1] = v.y;
+    } else {
+#pragma unroll
+        for (int k = 0; k < N / 16; ++k) {
+            const uint4 v = ((const uint4*)p)[k];
+            w[4 * k] = v.x; w[4 * k + 1] = v.y; w[4 * k + 2] = v.z; w[4 * k + 3] = v.w;
+        }
+    }
+}
+
+__device__ inline float max_over_quarters(float x) {       // over the four lanes that hold one query row
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ inline float sum_over_quarters(float x) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// How a row of DH channels is loaded: as the key operand (a quarter of the channels a lane, kKC loads of kKE) and as the value
+// operand (kVE consecutive channels of 8 keys).
+template <int DT, int STORE, int DH> struct Geo {
+    static constexpr bool kCodes = STORE != kStoreSame;
+    static constexpr int kBits = STORE == FF_STORE_E4M3 ? 8 : STORE == FF_STORE_E2M1 ? 4 : 8 * Act<DT>::kBytes;
+    static constexpr int kRow = DH * kBits / 8;
+    static constexpr int kKE = DH / 4 < 128 / kBits ? DH / 4 : 128 / kBits;
+    static constexpr int kKC = DH / 4 / kKE;
+    static constexpr int kKB = kKE * kBits / 8;
+    static constexpr int kKW = DH / 4 * kBits / 32;                    // words of a quarter row
+    static constexpr int kVE = DH / 16;
+    static constexpr int kVB = kVE * kBits / 8;
+    static constexpr int kVW = kVB < 4 ? 1 : kVB / 4;
+    static constexpr int kBlocks = DH / 32;                            // scale bytes of a row
+    static constexpr int kKSW = kBlocks < 4 ? 1 : kBlocks / 4;         // words of one row's scales
+    static constexpr int kVSW = kBlocks;                               // words of four rows' scales
+};
+
+// What a lane has loaded of 32 keys: quarter rows of keys (lane & 15) and 16 + (lane & 15); channels kVE (lane & 15) .. of keys
+// 4 q .. 4 q + 3 and 16 + 4 q .., q = lane >> 4; the scales of the same.
+template <int DT, int STORE, int DH> struct Raw {
+    using G = Geo<DT, STORE, DH>;
+    uint32_t k[2][G::kKW];
+    uint32_t v[8][G::kVW];
+    uint32_t ks[2][G::kCodes ? G::kKSW : 1];
+    uint32_t vs[2][G::kCodes ? G::kVSW : 1];
+};
+
+template <int DT, int STORE, int DH>
+__device__ inline void load_half(Raw<DT, STORE, DH>& raw, int sub, const ff_cache_t& c, int64_t row, int lane) {
+    using G = Geo<DT, STORE, DH>;
+    const int key = lane & 15, q = lane >> 4;
+    const char* k = (const char*)c.keys + row * G::kRow;
+    const char* v = (const char*)c.values + row * G::kRow;
+    const uint32_t ko = key * G::kRow + q * G::kKB, vo = 4 * q * G::kRow + key * G::kVB;
+#pragma unroll
+    for (int x = 0; x < G::kKC; ++x) load_words<G::kKB>(k + (ko + x * 4 * G::kKB), raw.k[sub] + x * (G::kKB / 4));
+#pragma unroll
+    for (int r = 0; r < 4; ++r) load_words<G::kVB>(v + (vo + r * G::kRow), raw.v[4 * sub + r]);
+    if constexpr (G::kCodes) {
+        load_words<G::kBlocks>((const char*)c.key_scales + row * G::kBlocks + key * G::kBlocks, raw.ks[sub]);
+        load_words<4 * G::kBlocks>((const char*)c.value_scales + row * G::kBlocks + 4 * q * G::kBlocks, raw.vs[sub]);
+    }
+}
+
+// 8 channels `step` of the quarter row
+template <int DT, int STORE, int DH> __device__ inline Frag<DT> key_frag(const Raw<DT, STORE, DH>& raw, int sub, int step, int lane) {
+    using G = Geo<DT, STORE, DH>;
+    Frag<DT> f;
+    if constexpr (!G::kCodes) {
+        if constexpr (DT == FF_F32) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f.w[e] = __uint_as_float(raw.k[sub][step * 8 + e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f.w[e] = raw.k[sub][step * 4 + e];
+        }
+    } else {
+        // block of the load this step belongs to: loads of 32 channels are blocks, of 16 halves, of 8 quarters of one
+        const int x = step * 8 / G::kKE, block = (x * 4 * G::kKE) / 32 + (lane >> 4) * G::kKE / 32;
+        const uint32_t word = G::kKSW == 1 ? raw.ks[sub][0] : (block >> 2 ? raw.ks[sub][G::kKSW - 1] : raw.ks[sub][0]);
+        const float scale = __uint_as_float(((word >> (8 * (block & 3))) & 255u) << 23);
+        constexpr int kPer = STORE == FF_STORE_E4M3 ? 2 : 4;          // pairs of a word
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t w = raw.k[sub][(step * 4 + e) / kPer];
+            if constexpr (DT == FF_F32) {
+                const f32x2 p = codes2_f32<STORE>(w, block_scale((word >> (8 * (block & 3))) & 255u), (step * 4 + e) % kPer);
+                f.w[2 * e] = p.x;
+                f.w[2 * e + 1] = p.y;
+            } else {
+                f.w[e] = codes2<DT, STORE>(w, scale, (step * 4 + e) % kPer);
+            }
+        }
+    }
+    return f;
+}
+// scale byte of key slot j for this lane's channels
+template <int DT, int STORE, int DH> __device__ inline uint32_t value_scale(const Raw<DT, STORE, DH>& raw, int j, int lane) {
+    using G = Geo<DT, STORE, DH>;
+    const int block = (lane & 15) * G::kVE / 32, r = j & 3, sub = j >> 2;
+    if constexpr (G::kBlocks == 8) {
+        const uint32_t w = block >> 2 ? raw.vs[sub][2 * r + 1] : raw.vs[sub][2 * r];
+        return (w >> (8 * (block & 3))) & 255u;
+    } else if constexpr (G::kBlocks == 4) {
+        return (raw.vs[sub][r] >> (8 * block)) & 255u;
+    } else if constexpr (G::kBlocks == 2) {
+        return (raw.vs[sub][r >> 1] >> (16 * (r & 1) + 8 * block)) & 255u;
+    } else {
+        return (raw.vs[sub][0] >> (8 * r)) & 255u;
+    }
+}
+
+// whether a value of this lane is NaN or infinite
+template <int DT, int STORE, int DH> __device__ inline bool values_not_finite(const Raw<DT, STORE, DH>& raw, int lane) {
+    using G = Geo<DT, STORE, DH>;
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        if constexpr (G::kCodes) bad |= value_scale<DT, STORE, DH>(raw, j, lane) == 255u;
+#pragma unroll
+        for (int y = 0; y < G::kVW; ++y) {
+            const uint32_t w = raw.v[j][y];
+            if constexpr (STORE == FF_STORE_E4M3) {                 // the code of all ones is NaN
+                bad |= (w & 0x7fu) == 0x7fu || (w & 0x7f00u) == 0x7f00u || (w & 0x7f0000u) == 0x7f0000u || (w & 0x7f000000u) == 0x7f000000u;
+            } else if constexpr (!G::kCodes) {
+                constexpr uint32_t kExp = DT == FF_F32 ? 0x7f800000u : DT == FF_BF16 ? 0x7f80u : 0x7c00u;
+                bad |= (w & kExp) == kExp || (DT != FF_F32 && (w & (kExp << 16)) == (kExp << 16));
+            }
+        }
+    }
+    return bad;
+}
+
+struct AttPlan {                    // what the host derives once a call
+    int G, R, groups;               // heads a kv head, query rows of one, workgroups over the rows
+    int splits, min_keys;           // workgroups over the keys at most; a workgroup takes at least so many
+    int page16;                     // page_size / 16 ...
+    uint32_t magic;                 // ... and floor(2^32 / page16) (2^32 - 1 for 1)
+    float scale2;                   // scale * log2(e)
+    float* part;                    // splits > 1: [B, kv heads, R, splits] x DH sums, then as many (maximum, sum) pairs
+    int64_t part_rows;
+};
+
+// splits really used for a sequence of `end` keys, and keys of each (a multiple of the tile)
+__device__ inline int used_splits(const AttPlan& p, int64_t end, int64_t& keys) {
+    int64_t s = (end + p.min_keys - 1) / p.min_keys;
+    s = s < 1 ? 1 : s > p.splits ? p.splits : s;
+    keys = ((end + s - 1) / s + kAttTile - 1) / kAttTile * kAttTile;
+    return (int)((end + keys - 1) / (keys ? keys : 1));
+}
+
+template <int DT, int STORE, int DH, int NT>
+__global__ __launch_bounds__(64 * kAttWaves, (DT == FF_F32 ? 2 : 1) * DH * NT > 256 ? 1 : 2) void k_cache_attention(const ff_cache_attention_t a, const AttPlan p) {
+    using G = Geo<DT, STORE, DH>;
+    constexpr int kSteps = DH / 32, kTiles = DH / 16, kPad = 4;
+    __shared__ float s_o[kAttWaves][16][DH + kPad];
+    __shared__ float s_m[kAttWaves][16], s_l[kAttWaves][16];
+    const ff_cache_t& c = a.cache;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), q = lane >> 4, col = lane & 15;
+    const int n = (int)c.n, kv = (int)c.kv_heads;
+    const int split = blockIdx.x, b = blockIdx.z, head = blockIdx.y / p.groups, group = blockIdx.y - head * p.groups;
+    const int64_t start = c.start[b];
+    const int64_t room = c.n_pages > 0 ? c.table_width * c.page_size : 0, end = start < 0 ? 0 : min(start + n, room);
+    int64_t keys;
+    const int used = used_splits(p, end, keys);
+    if (split >= used && split > 0) return;
+    const int64_t first = split * keys, last = min(end, first + keys);
+    const int32_t* table = c.table + (int64_t)b * c.table_width;
+
+    // the wave's rows of Q, NT tiles of 16; rows past R are zeros
+    Frag<DT> qf[NT][kSteps];
+    int token[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int r = (group * NT + t) * 16 + col;
+        token[t] = r / p.G;
+        const char* src = (const char*)a.q + ((int64_t)b * a.q_batch + (int64_t)(head * p.G + r - token[t] * p.G) * a.q_head + (int64_t)token[t] * a.q_token) * Act<DT>::kBytes;
+        // channels in the order of the keys' loads
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            constexpr int kQE = G::kKE < 8 ? G::kKE : 8;              // consecutive channels of a piece (fp32 keys: 4)
+#pragma unroll
+            for (int x = 0; x < 8 / kQE; ++x) {
+                const int at = s * 8 + x * kQE, load = at / G::kKE, d = load * 4 * G::kKE + q * G::kKE + at % G::kKE;
+                if constexpr (DT == FF_F32) {
+                    uint32_t w[kQE];
+                    if (r < p.R) {
+                        load_words<kQE * 4>(src + d * 4, w);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < kQE; ++e) w[e] = 0;
+                    }
+#pragma unroll
+                    for (int e = 0; e < kQE; ++e) qf[t][s].w[x * kQE + e] = __uint_as_float(w[e]);
+                } else {
+                    if (r < p.R) {
+                        load_words<16>(src + d * 2, qf[t][s].w);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) qf[t][s].w[e] = 0;
+                    }
+                }
+            }
+        }
+    }
+
+    f32x4 o[NT][kTiles];
+    float m[NT], l[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        m[t] = kNone;
+        l[t] = 0.f;
+#pragma unroll
+        for (int x = 0; x < kTiles; ++x) o[t][x] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // first row of 16 keys in the cache; -1: they have no place
+    auto row_of = [&](int64_t key) -> int64_t {
+        if (key >= end) return -1;
+        const uint32_t x = (uint32_t)(key >> 4);
+        uint32_t slot = __umulhi(x, p.magic), off = x - slot * p.page16;
+        if (off >= (uint32_t)p.page16) {
+            ++slot;
+            off -= p.page16;
+        }
+        const int page = table[slot];
+        if (page < 0 || page >= c.n_pages) return -1;
+        return ((int64_t)page * kv + head) * c.page_size + off * 16;
+    };
+    Raw<DT, STORE, DH> next;
+    int64_t next0 = -1, next1 = -1;
+    auto fetch = [&](int64_t key) {
+        next0 = row_of(key);
+        next1 = row_of(key + 16);
+        load_half<DT, STORE, DH>(next, 0, c, next0 < 0 ? 0 : next0, lane);      // (what has no place: any row, left out below)
+        load_half<DT, STORE, DH>(next, 1, c, next1 < 0 ? 0 : next1, lane);
+    };
+    const int64_t begin = first + wave * kAttTile;
+    if (begin < last) fetch(begin);
+    for (int64_t base = begin; base < last; base += kAttWaves * kAttTile) {
+        Raw<DT, STORE, DH> raw = next;
+        const int64_t row0 = next0, row1 = next1;
+        const bool have0 = row0 >= 0, have1 = row1 >= 0;
+        if (base + kAttWaves * kAttTile < last) fetch(base + kAttWaves * kAttTile);
+        const bool whole = have0 && have1 && base + kAttTile <= start;    // every row sees every key of the tile
+
+        f32x4 s[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+            for (int x = 0; x < kSteps; ++x) {
+                const Frag<DT> kf = key_frag<DT, STORE, DH>(raw, sub, x, lane);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) s[t][sub] = mma<DT>(kf, qf[t][x], s[t][sub]);
+            }
+        bool apart = false;
+        if (!whole) {
+            // values nobody sees may be anything: zeros stand in
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int64_t key = base + (j >> 2) * 16 + 4 * q + (j & 3);
+                if (!((j >> 2 ? have1 : have0) && key < end)) {
+#pragma unroll
+                    for (int y = 0; y < G::kVW; ++y) raw.v[j][y] = 0;
+                    if constexpr (G::kBlocks == 8) raw.vs[j >> 2][G::kCodes ? 2 * (j & 3) : 0] = raw.vs[j >> 2][G::kCodes ? 2 * (j & 3) + 1 : 0] = 0;
+                    else if constexpr (G::kBlocks == 4) raw.vs[j >> 2][G::kCodes ? j & 3 : 0] = 0;
+                    else if constexpr (G::kBlocks == 2) raw.vs[j >> 2][G::kCodes ? (j & 3) >> 1 : 0] &= j & 1 ? 0x0000ffffu : 0xffff0000u;
+                    else raw.vs[j >> 2][0] &= ~(255u << (8 * (j & 3)));
+                }
+            }
+            // new tokens do not all see each other: one's NaN or infinity must not reach those who do not (0 x NaN in the products)
+            apart = base + kAttTile > start && __any(values_not_finite<DT, STORE, DH>(raw, lane));
+        }
+        Frag<DT> pf[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            float x[8];
+            uint32_t sees = 255u;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = s[t][j >> 2][j & 3] * p.scale2;
+            if (!whole) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int64_t key = base + (j >> 2) * 16 + 4 * q + (j & 3);
+                    bool seen = (j >> 2 ? have1 : have0) && key < end && token[t] < n;
+                    if (seen && key >= start) {
+                        const int64_t fresh = key - start;
+                        seen = a.mask ? a.mask[(int64_t)b * a.mask_batch + (int64_t)token[t] * n + fresh] != 0 : fresh <= token[t];
+                    }
+                    x[j] = seen ? x[j] : kNone;
+                    if (!seen) sees &= ~(1u << j);
+                }
+            }
+            float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+            top = max_over_quarters(top);
+            // the running maximum moves only when a row passes it by 2^8: until then the weights stay below 256, nothing is lost
+            // and no output is rescaled
+            if (__any(top > m[t] + 8.f)) {
+                const float up = fmaxf(m[t], top), down = __builtin_amdgcn_exp2f(m[t] - (up == kNone ? 0.f : up));
+                m[t] = up;
+                l[t] *= down;
+#pragma unroll
+                for (int y = 0; y < kTiles; ++y) o[t][y] *= down;
+            }
+            const float zero = m[t] == kNone ? 0.f : m[t];
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                x[j] = __builtin_amdgcn_exp2f(x[j] - zero);
+                sum += x[j];
+            }
+            l[t] += sum;
+            if (apart) {
+                // rare: key by key in fp32, each row adding only what it sees.  The weights pass through the wave's part of s_o
+                float* weights = &s_o[wave][0][0];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) weights[((j >> 2) * 16 + 4 * q + (j & 3)) * 16 + col] = (sees >> j) & 1 ? x[j] : -1.f;
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 1
+                for (int k = 0; k < kAttTile; ++k) {
+                    const int64_t row = k < 16 ? row0 : row1;
+                    if (row < 0) continue;
+                    const float w = weights[k * 16 + col];
+                    if (w < 0.f) continue;
+#pragma unroll
+                    for (int u = 0; u < DH / 32; ++u) {
+                        float f[8];
+                        fetch8<DT, STORE>(c.values, c.value_scales, row + (k & 15), DH, q * (DH / 32) + u, f);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) o[t][(u * 8 + e) % kTiles][(u * 8 + e) / kTiles] = fmaf(w, f[e], o[t][(u * 8 + e) % kTiles][(u * 8 + e) / kTiles]);
+                    }
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            }
+            if constexpr (DT == FF_F32) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) pf[t].w[j] = x[j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) pf[t].w[j] = pack2<DT>(x[2 * j], x[2 * j + 1]);
+            }
+        }
+        if (apart) continue;
+        if constexpr (DT == FF_F32) {
+            Frag<DT> vf[kTiles];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if constexpr (G::kCodes) {
+                    const float scale = block_scale(value_scale<DT, STORE, DH>(raw, j, lane));
+                    constexpr int kPer = STORE == FF_STORE_E4M3 ? 2 : 4;
+#pragma unroll
+                    for (int y = 0; y < kTiles / 2; ++y) {
+                        const f32x2 v = codes2_f32<STORE>(raw.v[j][y / kPer], scale, y % kPer);
+                        vf[2 * y].w[j] = v.x;
+                        vf[2 * y + 1].w[j] = v.y;
+                    }
+                } else {
+#pragma unroll
+                    for (int y = 0; y < kTiles; ++y) vf[y].w[j] = __uint_as_float(raw.v[j][y]);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int y = 0; y < kTiles; ++y) o[t][y] = mma<DT>(vf[y], pf[t], o[t][y]);
+        } else {
+            float scale[8];
+            if constexpr (G::kCodes) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) scale[j] = __uint_as_float(value_scale<DT, STORE, DH>(raw, j, lane) << 23);
+            }
+            constexpr int kPer = STORE == FF_STORE_E4M3 ? 2 : 4;
+#pragma unroll
+            for (int y = 0; y < kTiles / 2; ++y) {
+                uint32_t w[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    if constexpr (G::kCodes) w[j] = codes2<DT, STORE>(raw.v[j][y / kPer], scale[j], y % kPer);
+                    else w[j] = raw.v[j][y];
+                }
+                Frag<DT> even, odd;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    even.w[e] = __builtin_amdgcn_perm(w[2 * e + 1], w[2 * e], 0x05040100u);
+                    odd.w[e] = __builtin_amdgcn_perm(w[2 * e + 1], w[2 * e], 0x07060302u);
+                }
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    o[t][2 * y] = mma<DT>(even, pf[t], o[t][2 * y]);
+                    o[t][2 * y + 1] = mma<DT>(odd, pf[t], o[t][2 * y + 1]);
+                }
+            }
+        }
+    }
+
+    // the four waves' rows, joined: channel (4 q + r) kVE + x of row `col` is o[x][r]
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        if (t) __syncthreads();
+        l[t] = sum_over_quarters(l[t]);
+        if (q == 0) {
+            s_m[wave][col] = m[t];
+            s_l[wave][col] = l[t];
+        }
+        __syncthreads();
+        float top = kNone;
+#pragma unroll
+        for (int w = 0; w < kAttWaves; ++w) top = fmaxf(top, s_m[w][col]);
+        const float down = __builtin_amdgcn_exp2f(m[t] - (top == kNone ? 0.f : top));
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int x = 0; x < kTiles; ++x) s_o[wave][col][(4 * q + r) * kTiles + x] = o[t][x][r] * down;
+        __syncthreads();
+        constexpr int kUnits = DH / 4;                                 // float4s of a row
+        for (int u = threadIdx.x; u < 16 * kUnits; u += 64 * kAttWaves) {
+            const int row = u / kUnits, d = (u - row * kUnits) * 4, r = (group * NT + t) * 16 + row;
+            if (r >= p.R) continue;
+            float most = kNone, sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < kAttWaves; ++w) most = fmaxf(most, s_m[w][row]);
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < kAttWaves; ++w) {
+                sum += s_l[w][row] * __builtin_amdgcn_exp2f(s_m[w][row] - (most == kNone ? 0.f : most));
+                acc += *(const f32x4*)&s_o[w][row][d];
+            }
+            if (p.splits > 1) {
+                const int64_t at = (((int64_t)b * kv + head) * p.R + r) * p.splits + split;
+                *(f32x4*)(p.part + at * DH + d) = acc;
+                if (d == 0) ((float2*)(p.part + p.part_rows * DH))[at] = make_float2(most, sum);
+            } else {
+                const int i = r / p.G;
+                char* out = (char*)a.out + ((int64_t)b * a.o_batch + (int64_t)(head * p.G + r - i * p.G) * a.o_head + (int64_t)i * a.o_token) * Act<DT>::kBytes;
+                const float over = sum == 0.f ? 0.f : 1.f / sum;       // (nothing seen: zeros)
+                if constexpr (DT == FF_F32) *(f32x4*)(out + d * 4) = acc * over;
+                else *(uint2*)(out + d * 2) = make_uint2(pack2<DT>(acc[0] * over, acc[1] * over), pack2<DT>(acc[2] * over, acc[3] * over));
+            }
+        }
+    }
+}
+
+// One workgroup joins the splits of one query row: thread (y, d) sums every kJoin-th split's channel d, the kJoin sums meet in
+// shared memory in fixed order.
+constexpr int kJoinThreads = 256;
+template <int DT, int DH>
+__global__ __launch_bounds__(kJoinThreads) void k_cache_attention_join(const ff_cache_attention_t a, const AttPlan p) {
+    constexpr int kUnits = DH / 4, kJoin = kJoinThreads / kUnits;
+    __shared__ f32x4 s_o[kJoin][kUnits];
+    __shared__ float s_l[kJoin];
+    __shared__ float s_top[kJoinThreads / 64];
+    const ff_cache_t& c = a.cache;
+    const int r = blockIdx.x, head = blockIdx.y, b = blockIdx.z, kv = (int)c.kv_heads, i = r / p.G;
+    const int64_t start = c.start[b];
+    const int64_t room = c.n_pages > 0 ? c.table_width * c.page_size : 0, end = start < 0 ? 0 : min(start + c.n, room);
+    int64_t keys;
+    const int used = max(1, used_splits(p, end, keys));
+    const int64_t at = (((int64_t)b * kv + head) * p.R + r) * p.splits;
+    const float2* ml = (const float2*)(p.part + p.part_rows * DH) + at;
+    const int u = threadIdx.x % kUnits, y = threadIdx.x / kUnits;
+    float top = kNone;
+    for (int s = threadIdx.x; s < used; s += kJoinThreads) top = fmaxf(top, ml[s].x);
+#pragma unroll
+    for (int k = 32; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor(top, k, 64));
+    if ((threadIdx.x & 63) == 0) s_top[threadIdx.x >> 6] = top;
+    __syncthreads();
+    top = s_top[0];
+#pragma unroll
+    for (int k = 1; k < kJoinThreads / 64; ++k) top = fmaxf(top, s_top[k]);
+    const float zero = top == kNone ? 0.f : top;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    float sum = 0.f;
+    for (int s = y; s < used; s += kJoin) {
+        const float2 x = ml[s];
+        const float w = __builtin_amdgcn_exp2f(x.x - zero);
+        acc += *(const f32x4*)(p.part + (at + s) * DH + u * 4) * w;
+        sum += x.y * w;
+    }
+    s_o[y][u] = acc;
+    if (u == 0) s_l[y] = sum;
+    __syncthreads();
+    if (y == 0) {
+        sum = s_l[0];
+#pragma unroll
+        for (int k = 1; k < kJoin; ++k) {
+            acc += s_o[k][u];
+            sum += s_l[k];
+        }
+        char* out = (char*)a.out + ((int64_t)b * a.o_batch + (int64_t)(head * p.G + r - i * p.G) * a.o_head + (int64_t)i * a.o_token) * Act<DT>::kBytes;
+        const float over = sum == 0.f ? 0.f : 1.f / sum;
+        if constexpr (DT == FF_F32) *(f32x4*)(out + u * 16) = acc * over;
+        else *(uint2*)(out + u * 8) = make_uint2(pack2<DT>(acc[0] * over, acc[1] * over), pack2<DT>(acc[2] * over, acc[3] * over));
+    }
 }
 
 static int attention_check(const ff_cache_attention_t* a) {
@@ -61,7 +605,7 @@ static int attention_check(const ff_cache_attention_t* a) {
     if (rc) return rc;
     if (!a->q || !a->out || a->H < 1 || a->H % a->cache.kv_heads || a->mask_batch < 0) return FF_ERR_ARG;
     if (a->cache.dh != 32 && a->cache.dh != 64 && a->cache.dh != 128 && a->cache.dh != 256) return FF_ERR_UNSUPPORTED;
-    if (a->H > 65535) return FF_ERR_UNSUPPORTED;
+    if (a->H > 65535 || a->cache.B > 65535 || a->cache.n * a->H > 65535 * 16) return FF_ERR_UNSUPPORTED;
     const int64_t per = a->cache.dtype == FF_F32 ? 4 : 8;
     if (!cache_aligned(a->q) || !cache_aligned(a->out)) return FF_ERR_ALIGN;
     const int64_t strides[6] = {a->q_batch, a->q_head, a->q_token, a->o_batch, a->o_head, a->o_token};
@@ -70,31 +614,76 @@ static int attention_check(const ff_cache_attention_t* a) {
     return FF_OK;
 }
 
-template <int DT, int STORE>
-static int launch_attention(const ff_cache_attention_t* a) {
-    k_cache_attention<DT, STORE><<<dim3((uint32_t)(a->cache.B * a->cache.n), (uint32_t)a->H), 64, 0, (hipStream_t)a->stream>>>(*a);
+// Tiles of 16 query rows a wave holds.  One when the rows fit one; four for the many rows of a tree or a chunk.
+static int row_tiles(int64_t R) { return R <= 16 ? 1 : R <= 32 ? 2 : 4; }
+
+static AttPlan attention_plan(const ff_cache_attention_t* a) {
+    const ff_cache_t& c = a->cache;
+    AttPlan p;
+    p.G = (int)(a->H / c.kv_heads);
+    p.R = (int)(p.G * c.n);
+    const int rows = 16 * row_tiles(p.R);
+    p.groups = (p.R + rows - 1) / rows;
+    p.page16 = (int)(c.page_size / 16);
+    p.magic = p.page16 == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / p.page16);
+    p.scale2 = (float)(a->scale * 1.4426950408889634);
+    p.min_keys = kAttWaves * kAttTile;
+    const int64_t base = c.B * c.kv_heads * p.groups, room = c.table_width * c.page_size;
+    int64_t s = (1024 + base - 1) / base;
+    const int64_t most = (room + p.min_keys - 1) / p.min_keys;
+    s = s < 1 ? 1 : s > 256 ? 256 : s;
+    if (s > most) s = most < 1 ? 1 : most;
+    p.splits = (int)s;
+    p.part_rows = s > 1 ? c.B * c.kv_heads * p.R * s : 0;
+    p.part = (float*)a->ws;
+    return p;
+}
+
+template <int DT, int STORE, int DH>
+static int launch_attention(const ff_cache_attention_t* a, const AttPlan& p) {
+    const ff_cache_t& c = a->cache;
+    const dim3 grid((uint32_t)p.splits, (uint32_t)(c.kv_heads * p.groups), (uint32_t)c.B);
+    hipStream_t st = (hipStream_t)a->stream;
+    switch (row_tiles(p.R)) {
+        case 1: k_cache_attention<DT, STORE, DH, 1><<<grid, 64 * kAttWaves, 0, st>>>(*a, p); break;
+        case 2: k_cache_attention<DT, STORE, DH, 2><<<grid, 64 * kAttWaves, 0, st>>>(*a, p); break;
+        default: k_cache_attention<DT, STORE, DH, 4><<<grid, 64 * kAttWaves, 0, st>>>(*a, p);
+    }
+    if (p.splits > 1) k_cache_attention_join<DT, DH><<<dim3((uint32_t)p.R, (uint32_t)c.kv_heads, (uint32_t)c.B), kJoinThreads, 0, st>>>(*a, p);
     return (int)hipGetLastError();
 }
+template <int DT, int STORE>
+static int launch_attention_dh(const ff_cache_attention_t* a, const AttPlan& p) {
+    switch (a->cache.dh) {
+        case 32: return launch_attention<DT, STORE, 32>(a, p);
+        case 64: return launch_attention<DT, STORE, 64>(a, p);
+        case 128: return launch_attention<DT, STORE, 128>(a, p);
+        default: return launch_attention<DT, STORE, 256>(a, p);
+    }
+}
 template <int DT>
-static int launch_attention_t(const ff_cache_attention_t* a) {
-    if (a->cache.store == FF_STORE_E4M3) return launch_attention<DT, FF_STORE_E4M3>(a);
-    if (a->cache.store == FF_STORE_E2M1) return launch_attention<DT, FF_STORE_E2M1>(a);
-    return launch_attention<DT, kStoreSame>(a);
+static int launch_attention_t(const ff_cache_attention_t* a, const AttPlan& p) {
+    if (a->cache.store == FF_STORE_E4M3) return launch_attention_dh<DT, FF_STORE_E4M3>(a, p);
+    if (a->cache.store == FF_STORE_E2M1) return launch_attention_dh<DT, FF_STORE_E2M1>(a, p);
+    return launch_attention_dh<DT, kStoreSame>(a, p);
 }
 
 }  // namespace ff
 
 extern "C" size_t ff_cache_attention_workspace_bytes(const ff_cache_attention_t* a) {
-    (void)a;
-    return 0;
+    if (ff::attention_check(a) || a->cache.B == 0 || a->cache.n == 0) return 0;
+    const ff::AttPlan p = ff::attention_plan(a);
+    return (size_t)p.part_rows * (size_t)(a->cache.dh + 2) * sizeof(float);
 }
 
 extern "C" int ff_cache_attention(const ff_cache_attention_t* a) {
     const int rc = ff::attention_check(a);
     if (rc) return rc;
     if (a->cache.B == 0 || a->cache.n == 0) return FF_OK;
-    if (a->ws_bytes < ff_cache_attention_workspace_bytes(a)) return FF_ERR_WORKSPACE;
-    if (a->cache.dtype == FF_F32) return ff::launch_attention_t<FF_F32>(a);
-    if (a->cache.dtype == FF_BF16) return ff::launch_attention_t<FF_BF16>(a);
-    return ff::launch_attention_t<FF_F16>(a);
+    const size_t need = ff_cache_attention_workspace_bytes(a);
+    if (a->ws_bytes < need || (need && (!a->ws || !ff::cache_aligned(a->ws)))) return FF_ERR_WORKSPACE;
+    const ff::AttPlan p = ff::attention_plan(a);
+    if (a->cache.dtype == FF_F32) return ff::launch_attention_t<FF_F32>(a, p);
+    if (a->cache.dtype == FF_BF16) return ff::launch_attention_t<FF_BF16>(a, p);
+    return ff::launch_attention_t<FF_F16>(a, p);
 }

@@ -16,7 +16,7 @@ int cache_check(const ff_cache_t* c) {
     if (!codes && c->store != c->dtype) return FF_ERR_ARG;
     if (codes && (!c->key_scales || !c->value_scales)) return FF_ERR_ARG;
     if (c->n_pages < 0 || c->kv_heads < 1 || c->page_size < 1 || c->dh < 1 || c->table_width < 0 || c->B < 0 || c->n < 0) return FF_ERR_ARG;
-    if (!cache_aligned(c->keys) || !cache_aligned(c->values)) return FF_ERR_ALIGN;
+    if (!cache_aligned(c->keys) || !cache_aligned(c->values) || !cache_aligned(c->key_scales) || !cache_aligned(c->value_scales)) return FF_ERR_ALIGN;
     if (c->dh % 32 || c->dh > 256 || c->page_size % 16 || c->page_size > 65536 || c->n_pages > 0x7fffffff || c->kv_heads > 4096) return FF_ERR_UNSUPPORTED;
     if (c->table_width > 0x7fff0000 / c->page_size) return FF_ERR_UNSUPPORTED;
     if (c->B > 0x7fffffff / 64 || c->n > 0x7fffffff / 64 || (c->n && c->B > 0x7fffffff / 64 / c->n)) return FF_ERR_UNSUPPORTED;
