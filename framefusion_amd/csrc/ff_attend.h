@@ -1,0 +1,102 @@
+// Shared by the two attention kernels over the paged cache: ff_attend.hip (few query rows) and ff_attend_rows.hip (many).
+#pragma once
+
+#include "ff_cache.h"
+
+namespace ff {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr float kNone = -__builtin_inff();
+
+template <int DT> __device__ inline uint32_t pack2(float a, float b) {      // two floats rounded to T (16 bits)
+    if constexpr (DT == FF_BF16) {
+        bf16x2_t p;
+        p.x = (__bf16)a;
+        p.y = (__bf16)b;
+        return __builtin_bit_cast(uint32_t, p);
+    } else {
+        half2_t p;
+        p.x = (_Float16)a;
+        p.y = (_Float16)b;
+        return __builtin_bit_cast(uint32_t, p);
+    }
+}
+// two codes of a stored word as T: 8 bits - pair `i` of 2, 4 bits - pair `i` of 4
+template <int DT, int STORE> __device__ inline uint32_t codes2(uint32_t w, float scale, int i) {
+    if constexpr (STORE == FF_STORE_E4M3) {
+        if constexpr (DT == FF_BF16)
+            return i ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true))
+                     : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false));
+        else
+            return i ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, true))
+                     : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, false));
+    } else {
+        if constexpr (DT == FF_BF16) {
+            return i == 0 ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0))
+                 : i == 1 ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1))
+                 : i == 2 ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2))
+                          : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3));
+        } else {
+            return i == 0 ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 0))
+                 : i == 1 ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 1))
+                 : i == 2 ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 2))
+                          : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 3));
+        }
+    }
+}
+struct AttPlan {                    // what the host derives once a call
+    int G, R, groups;               // heads a kv head, query rows of one (n G), workgroups over the rows
+    int splits, block;              // workgroups over the keys at most; split s takes blocks s, s + splits, .. of so many keys
+    int tiles;                      // many rows: tiles of 32 rows a workgroup
+    int page16;                     // page_size / 16 ...
+    uint32_t magic;                 // ... and floor(2^32 / page16) (2^32 - 1 for 1)
+    float scale2;                   // |scale| log2(e), at least the smallest normal number (0 times a masked score would be NaN)
+    uint32_t flip;                  // scale < 0: sign bits of two elements of 16-bit Q, taken up there (fp32: of one)
+    float* part;                    // splits > 1: [B, kv heads, R, splits] x DH sums, then as many (maximum, sum) pairs
+    int64_t part_rows;
+};
+
+// keys of a sequence that the new tokens may see: everything before them and themselves, as far as the table reaches
+__device__ inline int64_t keys_of(const ff_cache_t& c, int64_t start) {
+    const int64_t room = c.n_pages > 0 ? c.table_width * c.page_size : 0;
+    return start < 0 ? 0 : min(start + c.n, room);
+}
+// splits that have a block of a sequence of `end` keys (the first one answers for an empty sequence)
+__device__ inline int used_splits(const AttPlan& p, int64_t end) { return (int)max((int64_t)1, min((int64_t)p.splits, (end + p.block - 1) / p.block)); }
+
+// the page number (any value) of the 16 keys from `key` on, a multiple of 16, and their first row on it; -1 past the end
+__device__ inline int page_of_16(const AttPlan& p, const int32_t* table, int64_t key, int64_t end, int& off) {
+    const uint32_t x = (uint32_t)(key >> 4);
+    uint32_t slot = __umulhi(x, p.magic);                                      // (one too small at most)
+    off = x - slot * p.page16;
+    if (off >= p.page16) {
+        ++slot;
+        off -= p.page16;
+    }
+    off *= 16;
+    return key < end ? table[slot] : -1;
+}
+// row of the cache behind it for one kv head; -1: the keys have no place
+__device__ inline int64_t row_on_page(const ff_cache_t& c, int head, int page, int off) {
+    return page < 0 || page >= c.n_pages ? -1 : ((int64_t)page * (int)c.kv_heads + head) * c.page_size + off;
+}
+__device__ inline int64_t row_of_16(const ff_cache_t& c, const AttPlan& p, const int32_t* table, int head, int64_t key, int64_t end) {
+    int off;
+    const int page = page_of_16(p, table, key, end, off);
+    return row_on_page(c, head, page, off);
+}
+
+// four consecutive channels of one output row, sums divided by the weights' total (0: the row saw nothing)
+template <int DT> __device__ inline void write_out4(char* out, int d, f32x4 acc, float sum) {
+    const float over = sum == 0.f ? 0.f : 1.f / sum;
+    if constexpr (DT == FF_F32) *(f32x4*)(out + d * 4) = acc * over;
+    else *(uint2*)(out + d * 2) = make_uint2(pack2<DT>(acc[0] * over, acc[1] * over), pack2<DT>(acc[2] * over, acc[3] * over));
+}
+
+// csrc/ff_attend_rows.hip
+template <int DT> int launch_attention_rows(const ff_cache_attention_t* a, const AttPlan& p, int waves);
+
+}  // namespace ff

@@ -11,17 +11,12 @@
 // Codes become T by the scaled conversions of gfx950, one scale a block, exact (a code times a power of two fits T's mantissa).
 // The four waves of a workgroup take every fourth tile of 32 keys and are summed through shared memory; long caches are split over
 // workgroups, whose partial rows (maximum, sum, unscaled output, all fp32) a second launch joins in fixed order.
-#include "ff_cache.h"
+#include "ff_attend.h"
 
 namespace ff {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-
 constexpr int kAttWaves = 4;
 constexpr int kAttTile = 32;                       // keys of one step of a wave
-constexpr float kNone = -__builtin_inff();
 
 // ---- 8 elements of a lane in the operands of a product over 8 x 4 of them ------------------------------------------------
 template <int DT> struct Frag { uint32_t w[4]; };
@@ -39,42 +34,6 @@ template <int DT> __device__ inline f32x4 mma(const Frag<DT>& a, const Frag<DT>&
     }
 }
 
-template <int DT> __device__ inline uint32_t pack2(float a, float b) {      // two floats rounded to T (16 bits)
-    if constexpr (DT == FF_BF16) {
-        bf16x2_t p;
-        p.x = (__bf16)a;
-        p.y = (__bf16)b;
-        return __builtin_bit_cast(uint32_t, p);
-    } else {
-        half2_t p;
-        p.x = (_Float16)a;
-        p.y = (_Float16)b;
-        return __builtin_bit_cast(uint32_t, p);
-    }
-}
-// two codes of a stored word as T: 8 bits - pair `i` of 2, 4 bits - pair `i` of 4
-template <int DT, int STORE> __device__ inline uint32_t codes2(uint32_t w, float scale, int i) {
-    if constexpr (STORE == FF_STORE_E4M3) {
-        if constexpr (DT == FF_BF16)
-            return i ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true))
-                     : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false));
-        else
-            return i ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, true))
-                     : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, false));
-    } else {
-        if constexpr (DT == FF_BF16) {
-            return i == 0 ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0))
-                 : i == 1 ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1))
-                 : i == 2 ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2))
-                          : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3));
-        } else {
-            return i == 0 ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 0))
-                 : i == 1 ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 1))
-                 : i == 2 ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 2))
-                          : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 3));
-        }
-    }
-}
 template <int STORE> __device__ inline f32x2 codes2_f32(uint32_t w, float scale, int i) {
     f32x2 f;
     if constexpr (STORE == FF_STORE_E4M3) {
@@ -214,47 +173,46 @@ template <int DT, int STORE, int DH> __device__ inline uint32_t value_scale(cons
     }
 }
 
-// whether a value of this lane is NaN or infinite
-template <int DT, int STORE, int DH> __device__ inline bool values_not_finite(const Raw<DT, STORE, DH>& raw, int lane) {
+template <int DT, int STORE, int DH> __device__ inline void clear_value(Raw<DT, STORE, DH>& raw, int j) {
     using G = Geo<DT, STORE, DH>;
-    bool bad = false;
+#pragma unroll
+    for (int y = 0; y < G::kVW; ++y) raw.v[j][y] = 0;
+    if constexpr (G::kCodes) {
+        if constexpr (G::kBlocks == 8) raw.vs[j >> 2][2 * (j & 3)] = raw.vs[j >> 2][2 * (j & 3) + 1] = 0;
+        else if constexpr (G::kBlocks == 4) raw.vs[j >> 2][j & 3] = 0;
+        else if constexpr (G::kBlocks == 2) raw.vs[j >> 2][(j & 3) >> 1] &= j & 1 ? 0x0000ffffu : 0xffff0000u;
+        else raw.vs[j >> 2][0] &= ~(255u << (8 * (j & 3)));
+    }
+}
+// takes the NaN and infinities out of a lane's values; whether there were any
+template <int DT, int STORE, int DH> __device__ inline bool take_out_odd(Raw<DT, STORE, DH>& raw, int lane) {
+    using G = Geo<DT, STORE, DH>;
+    bool odd = false;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        if constexpr (G::kCodes) bad |= value_scale<DT, STORE, DH>(raw, j, lane) == 255u;
+        bool block = false;
+        if constexpr (G::kCodes) block = value_scale<DT, STORE, DH>(raw, j, lane) == 255u;
+        odd |= block;
+        if (block) clear_value<DT, STORE, DH>(raw, j);
 #pragma unroll
         for (int y = 0; y < G::kVW; ++y) {
-            const uint32_t w = raw.v[j][y];
+            uint32_t& w = raw.v[j][y];
             if constexpr (STORE == FF_STORE_E4M3) {                 // the code of all ones is NaN
-                bad |= (w & 0x7fu) == 0x7fu || (w & 0x7f00u) == 0x7f00u || (w & 0x7f0000u) == 0x7f0000u || (w & 0x7f000000u) == 0x7f000000u;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (((w >> (8 * k)) & 0x7fu) == 0x7fu) w &= ~(255u << (8 * k)), odd = true;
             } else if constexpr (!G::kCodes) {
                 constexpr uint32_t kExp = DT == FF_F32 ? 0x7f800000u : DT == FF_BF16 ? 0x7f80u : 0x7c00u;
-                bad |= (w & kExp) == kExp || (DT != FF_F32 && (w & (kExp << 16)) == (kExp << 16));
+                if ((w & kExp) == kExp) w = DT == FF_F32 ? 0u : w & 0xffff0000u, odd = true;
+                if (DT != FF_F32 && (w & (kExp << 16)) == (kExp << 16)) w &= 0xffffu, odd = true;
             }
         }
     }
-    return bad;
-}
-
-struct AttPlan {                    // what the host derives once a call
-    int G, R, groups;               // heads a kv head, query rows of one, workgroups over the rows
-    int splits, min_keys;           // workgroups over the keys at most; a workgroup takes at least so many
-    int page16;                     // page_size / 16 ...
-    uint32_t magic;                 // ... and floor(2^32 / page16) (2^32 - 1 for 1)
-    float scale2;                   // scale * log2(e)
-    float* part;                    // splits > 1: [B, kv heads, R, splits] x DH sums, then as many (maximum, sum) pairs
-    int64_t part_rows;
-};
-
-// splits really used for a sequence of `end` keys, and keys of each (a multiple of the tile)
-__device__ inline int used_splits(const AttPlan& p, int64_t end, int64_t& keys) {
-    int64_t s = (end + p.min_keys - 1) / p.min_keys;
-    s = s < 1 ? 1 : s > p.splits ? p.splits : s;
-    keys = ((end + s - 1) / s + kAttTile - 1) / kAttTile * kAttTile;
-    return (int)((end + keys - 1) / (keys ? keys : 1));
+    return odd;
 }
 
 template <int DT, int STORE, int DH, int NT>
-__global__ __launch_bounds__(64 * kAttWaves, (DT == FF_F32 ? 2 : 1) * DH * NT > 256 ? 1 : 2) void k_cache_attention(const ff_cache_attention_t a, const AttPlan p) {
+__global__ __launch_bounds__(64 * kAttWaves, DH * NT * (STORE == kStoreSame ? Act<DT>::kBytes : 2) >= 512 ? 1 : 2) void k_cache_attention(const ff_cache_attention_t a, const AttPlan p) {
     using G = Geo<DT, STORE, DH>;
     constexpr int kSteps = DH / 32, kTiles = DH / 16, kPad = 4;
     __shared__ float s_o[kAttWaves][16][DH + kPad];
@@ -264,11 +222,8 @@ __global__ __launch_bounds__(64 * kAttWaves, (DT == FF_F32 ? 2 : 1) * DH * NT > 
     const int n = (int)c.n, kv = (int)c.kv_heads;
     const int split = blockIdx.x, b = blockIdx.z, head = blockIdx.y / p.groups, group = blockIdx.y - head * p.groups;
     const int64_t start = c.start[b];
-    const int64_t room = c.n_pages > 0 ? c.table_width * c.page_size : 0, end = start < 0 ? 0 : min(start + n, room);
-    int64_t keys;
-    const int used = used_splits(p, end, keys);
-    if (split >= used && split > 0) return;
-    const int64_t first = split * keys, last = min(end, first + keys);
+    const int64_t end = keys_of(c, start);
+    if (split >= used_splits(p, end)) return;
     const int32_t* table = c.table + (int64_t)b * c.table_width;
 
     // the wave's rows of Q, NT tiles of 16; rows past R are zeros
@@ -295,10 +250,12 @@ __global__ __launch_bounds__(64 * kAttWaves, (DT == FF_F32 ? 2 : 1) * DH * NT > 
                         for (int e = 0; e < kQE; ++e) w[e] = 0;
                     }
 #pragma unroll
-                    for (int e = 0; e < kQE; ++e) qf[t][s].w[x * kQE + e] = __uint_as_float(w[e]);
+                    for (int e = 0; e < kQE; ++e) qf[t][s].w[x * kQE + e] = __uint_as_float(w[e] ^ p.flip);
                 } else {
                     if (r < p.R) {
                         load_words<16>(src + d * 2, qf[t][s].w);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) qf[t][s].w[e] ^= p.flip;
                     } else {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) qf[t][s].w[e] = 0;
@@ -318,34 +275,35 @@ __global__ __launch_bounds__(64 * kAttWaves, (DT == FF_F32 ? 2 : 1) * DH * NT > 
         for (int x = 0; x < kTiles; ++x) o[t][x] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
-    // first row of 16 keys in the cache; -1: they have no place
-    auto row_of = [&](int64_t key) -> int64_t {
-        if (key >= end) return -1;
-        const uint32_t x = (uint32_t)(key >> 4);
-        uint32_t slot = __umulhi(x, p.magic), off = x - slot * p.page16;
-        if (off >= (uint32_t)p.page16) {
-            ++slot;
-            off -= p.page16;
-        }
-        const int page = table[slot];
-        if (page < 0 || page >= c.n_pages) return -1;
-        return ((int64_t)page * kv + head) * c.page_size + off * 16;
-    };
     Raw<DT, STORE, DH> next;
     int64_t next0 = -1, next1 = -1;
-    auto fetch = [&](int64_t key) {
-        next0 = row_of(key);
-        next1 = row_of(key + 16);
+    int page0 = -1, page1 = -1, off0 = 0, off1 = 0;
+    auto look_up = [&](int64_t key) {             // the pages of a tile, a tile before its rows are loaded
+        page0 = page_of_16(p, table, key, end, off0);
+        page1 = page_of_16(p, table, key + 16, end, off1);
+    };
+    auto fetch = [&]() {
+        next0 = row_on_page(c, head, page0, off0);
+        next1 = row_on_page(c, head, page1, off1);
         load_half<DT, STORE, DH>(next, 0, c, next0 < 0 ? 0 : next0, lane);      // (what has no place: any row, left out below)
         load_half<DT, STORE, DH>(next, 1, c, next1 < 0 ? 0 : next1, lane);
     };
-    const int64_t begin = first + wave * kAttTile;
-    if (begin < last) fetch(begin);
-    for (int64_t base = begin; base < last; base += kAttWaves * kAttTile) {
+    const uint8_t* mask = a.mask ? a.mask + (int64_t)b * a.mask_batch : nullptr;
+    bool odd = false;
+    const int64_t begin = ((int64_t)split * kAttWaves + wave) * kAttTile, stride = (int64_t)p.splits * kAttWaves * kAttTile;
+    if (begin < end) {
+        look_up(begin);
+        fetch();
+        look_up(begin + stride);
+    }
+    for (int64_t base = begin; base < end; base += stride) {
         Raw<DT, STORE, DH> raw = next;
         const int64_t row0 = next0, row1 = next1;
         const bool have0 = row0 >= 0, have1 = row1 >= 0;
-        if (base + kAttWaves * kAttTile < last) fetch(base + kAttWaves * kAttTile);
+        if (base + stride < end) {
+            fetch();
+            look_up(base + 2 * stride);
+        }
         const bool whole = have0 && have1 && base + kAttTile <= start;    // every row sees every key of the tile
 
         f32x4 s[NT][2];
@@ -359,46 +317,40 @@ __global__ __launch_bounds__(64 * kAttWaves, (DT == FF_F32 ? 2 : 1) * DH * NT > 
 #pragma unroll
                 for (int t = 0; t < NT; ++t) s[t][sub] = mma<DT>(kf, qf[t][x], s[t][sub]);
             }
-        bool apart = false;
         if (!whole) {
             // values nobody sees may be anything: zeros stand in
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int64_t key = base + (j >> 2) * 16 + 4 * q + (j & 3);
-                if (!((j >> 2 ? have1 : have0) && key < end)) {
-#pragma unroll
-                    for (int y = 0; y < G::kVW; ++y) raw.v[j][y] = 0;
-                    if constexpr (G::kBlocks == 8) raw.vs[j >> 2][G::kCodes ? 2 * (j & 3) : 0] = raw.vs[j >> 2][G::kCodes ? 2 * (j & 3) + 1 : 0] = 0;
-                    else if constexpr (G::kBlocks == 4) raw.vs[j >> 2][G::kCodes ? j & 3 : 0] = 0;
-                    else if constexpr (G::kBlocks == 2) raw.vs[j >> 2][G::kCodes ? (j & 3) >> 1 : 0] &= j & 1 ? 0x0000ffffu : 0xffff0000u;
-                    else raw.vs[j >> 2][0] &= ~(255u << (8 * (j & 3)));
-                }
-            }
-            // new tokens do not all see each other: one's NaN or infinity must not reach those who do not (0 x NaN in the products)
-            apart = base + kAttTile > start && __any(values_not_finite<DT, STORE, DH>(raw, lane));
+            for (int j = 0; j < 8; ++j)
+                if (!((j >> 2 ? have1 : have0) && base + (j >> 2) * 16 + 4 * q + (j & 3) < end)) clear_value<DT, STORE, DH>(raw, j);
+            // new tokens do not all see each other, and 0 x NaN is NaN: a NaN or infinity among these keys' values stays out of the
+            // products and is added at the end to the rows that see it
+            if (base + kAttTile > start && take_out_odd<DT, STORE, DH>(raw, lane)) odd = true;
         }
         Frag<DT> pf[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             float x[8];
-            uint32_t sees = 255u;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = s[t][j >> 2][j & 3] * p.scale2;
+            for (int j = 0; j < 8; ++j) x[j] = s[t][j >> 2][j & 3];
             if (!whole) {
+                const int fresh0 = (int)(base - start) + 4 * q, left = (int)(end - base) - 4 * q, own = min(token[t], n - 1);
+                uint32_t sees = 0;
+                if (mask) {
+                    uint32_t byte[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int64_t key = base + (j >> 2) * 16 + 4 * q + (j & 3);
-                    bool seen = (j >> 2 ? have1 : have0) && key < end && token[t] < n;
-                    if (seen && key >= start) {
-                        const int64_t fresh = key - start;
-                        seen = a.mask ? a.mask[(int64_t)b * a.mask_batch + (int64_t)token[t] * n + fresh] != 0 : fresh <= token[t];
-                    }
-                    x[j] = seen ? x[j] : kNone;
-                    if (!seen) sees &= ~(1u << j);
+                    for (int j = 0; j < 8; ++j) byte[j] = mask[(int64_t)own * n + min(max(fresh0 + (j >> 2) * 16 + (j & 3), 0), n - 1)];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) sees |= byte[j] || fresh0 + (j >> 2) * 16 + (j & 3) < 0 ? 1u << j : 0u;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) sees |= fresh0 + (j >> 2) * 16 + (j & 3) <= own ? 1u << j : 0u;
                 }
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (!((sees >> j) & 1u) || !(j >> 2 ? have1 : have0) || (j >> 2) * 16 + (j & 3) >= left) x[j] = kNone;
             }
             float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-            top = max_over_quarters(top);
+            top = max_over_quarters(top) * p.scale2;
             // the running maximum moves only when a row passes it by 2^8: until then the weights stay below 256, nothing is lost
             // and no output is rescaled
             if (__any(top > m[t] + 8.f)) {
@@ -412,32 +364,10 @@ __global__ __launch_bounds__(64 * kAttWaves, (DT == FF_F32 ? 2 : 1) * DH * NT > 
             float sum = 0.f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                x[j] = __builtin_amdgcn_exp2f(x[j] - zero);
+                x[j] = __builtin_amdgcn_exp2f(fmaf(x[j], p.scale2, -zero));
                 sum += x[j];
             }
             l[t] += sum;
-            if (apart) {
-                // rare: key by key in fp32, each row adding only what it sees.  The weights pass through the wave's part of s_o
-                float* weights = &s_o[wave][0][0];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) weights[((j >> 2) * 16 + 4 * q + (j & 3)) * 16 + col] = (sees >> j) & 1 ? x[j] : -1.f;
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll 1
-                for (int k = 0; k < kAttTile; ++k) {
-                    const int64_t row = k < 16 ? row0 : row1;
-                    if (row < 0) continue;
-                    const float w = weights[k * 16 + col];
-                    if (w < 0.f) continue;
-#pragma unroll
-                    for (int u = 0; u < DH / 32; ++u) {
-                        float f[8];
-                        fetch8<DT, STORE>(c.values, c.value_scales, row + (k & 15), DH, q * (DH / 32) + u, f);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) o[t][(u * 8 + e) % kTiles][(u * 8 + e) / kTiles] = fmaf(w, f[e], o[t][(u * 8 + e) % kTiles][(u * 8 + e) / kTiles]);
-                    }
-                }
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            }
             if constexpr (DT == FF_F32) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) pf[t].w[j] = x[j];
@@ -446,7 +376,6 @@ __global__ __launch_bounds__(64 * kAttWaves, (DT == FF_F32 ? 2 : 1) * DH * NT > 
                 for (int j = 0; j < 4; ++j) pf[t].w[j] = pack2<DT>(x[2 * j], x[2 * j + 1]);
             }
         }
-        if (apart) continue;
         if constexpr (DT == FF_F32) {
             Frag<DT> vf[kTiles];
 #pragma unroll
@@ -499,6 +428,34 @@ __global__ __launch_bounds__(64 * kAttWaves, (DT == FF_F32 ? 2 : 1) * DH * NT > 
         }
     }
 
+    if (__any(odd)) {
+        // rare: the values left out above, to the rows that see them (their weight is positive: infinities and NaN stay what they are)
+        for (int64_t base = begin; base < end; base += stride) {
+            if (base + kAttTile <= start) continue;
+#pragma unroll 1
+            for (int k = 0; k < kAttTile; ++k) {
+                const int64_t r = row_of_16(c, p, table, head, base + (k & 16), end), fresh = base + k - start;
+                if (r < 0 || base + k >= end) continue;
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const int own = min(token[t], n - 1);
+                    if (fresh >= 0 && !(mask ? mask[(int64_t)own * n + fresh] != 0 : fresh <= own)) continue;
+#pragma unroll
+                    for (int u = 0; u < DH / 32; ++u) {
+                        float f[8];
+                        __builtin_amdgcn_sched_barrier(0);             // (one load at a time: registers are for the usual path)
+                        fetch8<DT, STORE>(c.values, c.value_scales, r + (k & 15), DH, q * (DH / 32) + u, f);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const float v = Act<DT>::rnd(f[e]);
+                            if (!(fabsf(v) < __builtin_inff())) o[t][(u * 8 + e) % kTiles][(u * 8 + e) / kTiles] += v;
+                        }
+                    }
+                }
+            }
+        }
+    }
+
     // the four waves' rows, joined: channel (4 q + r) kVE + x of row `col` is o[x][r]
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -538,9 +495,7 @@ __global__ __launch_bounds__(64 * kAttWaves, (DT == FF_F32 ? 2 : 1) * DH * NT > 
             } else {
                 const int i = r / p.G;
                 char* out = (char*)a.out + ((int64_t)b * a.o_batch + (int64_t)(head * p.G + r - i * p.G) * a.o_head + (int64_t)i * a.o_token) * Act<DT>::kBytes;
-                const float over = sum == 0.f ? 0.f : 1.f / sum;       // (nothing seen: zeros)
-                if constexpr (DT == FF_F32) *(f32x4*)(out + d * 4) = acc * over;
-                else *(uint2*)(out + d * 2) = make_uint2(pack2<DT>(acc[0] * over, acc[1] * over), pack2<DT>(acc[2] * over, acc[3] * over));
+                write_out4<DT>(out, d, acc, sum);
             }
         }
     }
@@ -557,10 +512,7 @@ __global__ __launch_bounds__(kJoinThreads) void k_cache_attention_join(const ff_
     __shared__ float s_top[kJoinThreads / 64];
     const ff_cache_t& c = a.cache;
     const int r = blockIdx.x, head = blockIdx.y, b = blockIdx.z, kv = (int)c.kv_heads, i = r / p.G;
-    const int64_t start = c.start[b];
-    const int64_t room = c.n_pages > 0 ? c.table_width * c.page_size : 0, end = start < 0 ? 0 : min(start + c.n, room);
-    int64_t keys;
-    const int used = max(1, used_splits(p, end, keys));
+    const int used = used_splits(p, keys_of(c, c.start[b]));
     const int64_t at = (((int64_t)b * kv + head) * p.R + r) * p.splits;
     const float2* ml = (const float2*)(p.part + p.part_rows * DH) + at;
     const int u = threadIdx.x % kUnits, y = threadIdx.x / kUnits;
@@ -593,9 +545,7 @@ __global__ __launch_bounds__(kJoinThreads) void k_cache_attention_join(const ff_
             sum += s_l[k];
         }
         char* out = (char*)a.out + ((int64_t)b * a.o_batch + (int64_t)(head * p.G + r - i * p.G) * a.o_head + (int64_t)i * a.o_token) * Act<DT>::kBytes;
-        const float over = sum == 0.f ? 0.f : 1.f / sum;
-        if constexpr (DT == FF_F32) *(f32x4*)(out + u * 16) = acc * over;
-        else *(uint2*)(out + u * 8) = make_uint2(pack2<DT>(acc[0] * over, acc[1] * over), pack2<DT>(acc[2] * over, acc[3] * over));
+        write_out4<DT>(out, u * 4, acc, sum);
     }
 }
 
@@ -614,23 +564,38 @@ static int attention_check(const ff_cache_attention_t* a) {
     return FF_OK;
 }
 
-// Tiles of 16 query rows a wave holds.  One when the rows fit one; four for the many rows of a tree or a chunk.
-static int row_tiles(int64_t R) { return R <= 16 ? 1 : R <= 32 ? 2 : 4; }
+// Which kernel serves R query rows, and how many waves share a block of keys.  Up to 32 rows (and fp32, whose products are slow
+// anyway): ff_attend.hip, tiles of 16 rows; more: ff_attend_rows.hip, tiles of 32 rows, a wave each.
+static int row_waves(int dtype, int64_t R, int64_t dh) {
+    if (dtype == FF_F32 || R <= 32) return 0;
+    return R <= 64 ? 2 : R <= 128 || dh == 256 ? 4 : 8;
+}
 
 static AttPlan attention_plan(const ff_cache_attention_t* a) {
     const ff_cache_t& c = a->cache;
     AttPlan p;
     p.G = (int)(a->H / c.kv_heads);
     p.R = (int)(p.G * c.n);
-    const int rows = 16 * row_tiles(p.R);
-    p.groups = (p.R + rows - 1) / rows;
+    const int waves = row_waves((int)c.dtype, p.R, c.dh);
+    if (waves) {
+        const int tiles = (p.R + 31) / 32;
+        p.groups = (tiles + waves - 1) / waves;
+        p.tiles = (tiles + p.groups - 1) / p.groups;
+        p.block = 64;
+    } else {
+        // two tiles of 16 rows a wave where their registers fit beside the keys' (16-bit T up to 128 channels, fp32 up to 64)
+        p.tiles = p.R <= 16 || c.dh > (c.dtype == FF_F32 ? 64 : 128) ? 1 : 2;
+        p.groups = (p.R + 16 * p.tiles - 1) / (16 * p.tiles);
+        p.block = kAttWaves * kAttTile;
+    }
     p.page16 = (int)(c.page_size / 16);
     p.magic = p.page16 == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / p.page16);
-    p.scale2 = (float)(a->scale * 1.4426950408889634);
-    p.min_keys = kAttWaves * kAttTile;
+    const double scale2 = a->scale * 1.4426950408889634;
+    p.scale2 = fmaxf(fabsf((float)scale2), 1.17549435e-38f);
+    p.flip = scale2 < 0 ? (c.dtype == FF_F32 ? 0x80000000u : 0x80008000u) : 0u;
     const int64_t base = c.B * c.kv_heads * p.groups, room = c.table_width * c.page_size;
-    int64_t s = (1024 + base - 1) / base;
-    const int64_t most = (room + p.min_keys - 1) / p.min_keys;
+    int64_t s = ((waves ? 2048 / waves : 1024) + base - 1) / base;
+    const int64_t most = (room + p.block - 1) / p.block;
     s = s < 1 ? 1 : s > 256 ? 256 : s;
     if (s > most) s = most < 1 ? 1 : most;
     p.splits = (int)s;
@@ -644,12 +609,9 @@ static int launch_attention(const ff_cache_attention_t* a, const AttPlan& p) {
     const ff_cache_t& c = a->cache;
     const dim3 grid((uint32_t)p.splits, (uint32_t)(c.kv_heads * p.groups), (uint32_t)c.B);
     hipStream_t st = (hipStream_t)a->stream;
-    switch (row_tiles(p.R)) {
-        case 1: k_cache_attention<DT, STORE, DH, 1><<<grid, 64 * kAttWaves, 0, st>>>(*a, p); break;
-        case 2: k_cache_attention<DT, STORE, DH, 2><<<grid, 64 * kAttWaves, 0, st>>>(*a, p); break;
-        default: k_cache_attention<DT, STORE, DH, 4><<<grid, 64 * kAttWaves, 0, st>>>(*a, p);
-    }
-    if (p.splits > 1) k_cache_attention_join<DT, DH><<<dim3((uint32_t)p.R, (uint32_t)c.kv_heads, (uint32_t)c.B), kJoinThreads, 0, st>>>(*a, p);
+    if constexpr (DH <= (DT == FF_F32 ? 64 : 128))
+        if (p.tiles == 2) k_cache_attention<DT, STORE, DH, 2><<<grid, 64 * kAttWaves, 0, st>>>(*a, p);
+    if (p.tiles == 1) k_cache_attention<DT, STORE, DH, 1><<<grid, 64 * kAttWaves, 0, st>>>(*a, p);
     return (int)hipGetLastError();
 }
 template <int DT, int STORE>
@@ -661,11 +623,28 @@ static int launch_attention_dh(const ff_cache_attention_t* a, const AttPlan& p) 
         default: return launch_attention<DT, STORE, 256>(a, p);
     }
 }
+template <int DT, int DH>
+static int launch_join(const ff_cache_attention_t* a, const AttPlan& p) {
+    k_cache_attention_join<DT, DH><<<dim3((uint32_t)p.R, (uint32_t)a->cache.kv_heads, (uint32_t)a->cache.B), kJoinThreads, 0, (hipStream_t)a->stream>>>(*a, p);
+    return (int)hipGetLastError();
+}
 template <int DT>
 static int launch_attention_t(const ff_cache_attention_t* a, const AttPlan& p) {
-    if (a->cache.store == FF_STORE_E4M3) return launch_attention_dh<DT, FF_STORE_E4M3>(a, p);
-    if (a->cache.store == FF_STORE_E2M1) return launch_attention_dh<DT, FF_STORE_E2M1>(a, p);
-    return launch_attention_dh<DT, kStoreSame>(a, p);
+    const int waves = row_waves(DT, p.R, a->cache.dh);
+    int rc;
+    if constexpr (DT != FF_F32) rc = waves ? launch_attention_rows<DT>(a, p, waves) : FF_OK;
+    if (!waves) {
+        if (a->cache.store == FF_STORE_E4M3) rc = launch_attention_dh<DT, FF_STORE_E4M3>(a, p);
+        else if (a->cache.store == FF_STORE_E2M1) rc = launch_attention_dh<DT, FF_STORE_E2M1>(a, p);
+        else rc = launch_attention_dh<DT, kStoreSame>(a, p);
+    }
+    if (rc || p.splits == 1) return rc;
+    switch (a->cache.dh) {
+        case 32: return launch_join<DT, 32>(a, p);
+        case 64: return launch_join<DT, 64>(a, p);
+        case 128: return launch_join<DT, 128>(a, p);
+        default: return launch_join<DT, 256>(a, p);
+    }
 }
 
 }  // namespace ff

@@ -1,0 +1,346 @@
+// ff_attend_rows.hip - attention of many query rows (a tree or a chunk of new tokens, times the heads of a kv head) over the paged
+// cache, for 16-bit T.
+//
+// With more than 32 rows the products, not the cache's bytes, are what costs, so keys and values are made ready ONCE for all
+// waves of a workgroup: 64 keys at a time are loaded, turned into T (codes) and laid in shared memory row by row; two buffers, the
+// next 64 keys in flight in registers meanwhile (and the page numbers of those behind them), one barrier a step.  A wave owns 32
+// rows: S^T = K Q^T leaves a lane with 16 of 32 keys of ONE row (its other half in lane + 32), which is also what O^T = V^T P^T
+// wants, so the weights never leave the registers; V^T comes out of shared memory by the transposing reads (ds_read_b64_tr_b16:
+// 16 lanes that point at 4 rows of 16 channels get one channel of 4 rows each).  Shared memory is read at 128 bytes a clock and a
+// CU's four matrix pipes ask for exactly that at 32 rows a wave; the softmax (one exponential a score at a quarter of the
+// rate) costs as much again and runs beside the products of the other wave of the SIMD.
+#include <atomic>
+
+#include "ff_attend.h"
+
+namespace ff {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kRowsKeys = 64;                 // keys of a step
+
+template <int DT> __device__ inline f32x16 mma32(const uint4& a, const uint4& b, f32x16 c) {
+    if constexpr (DT == FF_BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+
+// 16 channels x 4 rows: lane i of 16 points at channels 4 (i % 4) of row i / 4 and gets channel i of the rows
+__device__ inline uint2 read_turned(const char* p) { return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(p))); }
+
+template <int DT, int STORE, int DH, int NW>
+__global__ __launch_bounds__(64 * NW, DH == 256 || NW == 2 ? 1 : 2) void k_cache_attention_rows(const ff_cache_attention_t a, const AttPlan p) {
+    constexpr int kThreads = 64 * NW, kSteps = DH / 16, kTiles = DH / 32;
+    constexpr int kStride = DH * 2 + 16;                                             // bytes of a row in shared memory; the 16 spread the banks
+    constexpr int kBuf = 2 * kRowsKeys * kStride;                                    // keys, then values
+    // a unit of the loading: 32 channels of one key or value
+    constexpr int kUnits = 4 * DH, kMine = (kUnits + kThreads - 1) / kThreads, kWords = STORE == kStoreSame ? 16 : STORE == FF_STORE_E4M3 ? 8 : 4;
+    constexpr int kRow = STORE == FF_STORE_E4M3 ? DH : STORE == FF_STORE_E2M1 ? DH / 2 : 2 * DH;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ int s_odd;                     // a value of the keys from the new tokens on is NaN or infinite
+    __shared__ int s_have[2][4];              // which 16 keys of a buffer have a place
+    const ff_cache_t& c = a.cache;
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), h = lane >> 5, col = lane & 31;
+    const int n = (int)c.n, kv = (int)c.kv_heads;
+    const int split = blockIdx.x, b = blockIdx.z, head = blockIdx.y / p.groups, group = blockIdx.y - head * p.groups;
+    const int64_t start = c.start[b], end = keys_of(c, start);
+    if (split >= used_splits(p, end)) return;
+    const int32_t* table = c.table + (int64_t)b * c.table_width;
+    if (tid == 0) s_odd = 0;
+
+    // the wave's 32 rows of Q; a wave behind the group's last tile only loads
+    const int tile = group * p.tiles + wave, row = tile * 32 + col;
+    const bool works = wave < p.tiles && tile * 32 < p.R;
+    const int token = row / p.G;
+    uint4 qf[kSteps];
+    {
+        const char* src = (const char*)a.q + ((int64_t)b * a.q_batch + (int64_t)(head * p.G + row - token * p.G) * a.q_head + (int64_t)token * a.q_token) * 2;
+#pragma unroll
+        for (int x = 0; x < kSteps; ++x) qf[x] = make_uint4(0, 0, 0, 0);
+        if (works && row < p.R) {
+#pragma unroll
+            for (int x = 0; x < kSteps; ++x) {
+                const uint4 v = *(const uint4*)(src + (x * 16 + h * 8) * 2);
+                qf[x] = make_uint4(v.x ^ p.flip, v.y ^ p.flip, v.z ^ p.flip, v.w ^ p.flip);
+            }
+        }
+    }
+    f32x16 o[kTiles];
+#pragma unroll
+    for (int y = 0; y < kTiles; ++y)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[y][e] = 0.f;
+    float m = kNone, l = 0.f;
+
+    // ---- unit u = tid + i kThreads: block x of key (u mod 2 DH) / (DH / 32), of the keys for u < 2 DH, else of the values
+    uint32_t w[kMine][kWords], sc[kMine];
+    int page[kMine], page_next[kMine];
+    auto key_of = [&](int i) { return ((tid + i * kThreads) % (2 * DH)) / (DH / 32); };
+    auto look_up = [&](int64_t base) {           // the pages of a step, a step before its rows are loaded
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            const int64_t at = base + key_of(i);
+            const uint32_t x = (uint32_t)(at >> 4);
+            uint32_t slot = __umulhi(x, p.magic);
+            slot += x - slot * p.page16 >= (uint32_t)p.page16;
+            page_next[i] = at < end ? table[slot] : -1;      // (looked at only when the rows are loaded)
+        }
+    };
+    auto fetch = [&](int64_t base) {
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            page[i] = page_next[i] < c.n_pages ? page_next[i] : -1;
+            const int u = tid + i * kThreads;
+            if (kUnits % kThreads && u >= kUnits) continue;
+            const uint32_t at = (uint32_t)(base + key_of(i));
+            uint32_t q = __umulhi(at >> 4, p.magic);
+            q += (at >> 4) - q * p.page16 >= (uint32_t)p.page16;
+            const int64_t row = page[i] < 0 ? 0 : ((int64_t)page[i] * kv + head) * c.page_size + (at - q * (uint32_t)c.page_size);   // (no place: any row, left out below)
+            const int x = u % (DH / 32);
+            const bool is_v = u >= 2 * DH;
+            const char* src = (const char*)(is_v ? c.values : c.keys) + row * kRow;
+            if constexpr (STORE == kStoreSame) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint4 v = ((const uint4*)src)[k * (DH / 32) + x];          // (16 bytes of neighbours side by side)
+                    w[i][4 * k] = v.x; w[i][4 * k + 1] = v.y; w[i][4 * k + 2] = v.z; w[i][4 * k + 3] = v.w;
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < kWords / 4; ++k) {
+                    const uint4 v = ((const uint4*)src)[x * (kWords / 4) + k];
+                    w[i][4 * k] = v.x; w[i][4 * k + 1] = v.y; w[i][4 * k + 2] = v.z; w[i][4 * k + 3] = v.w;
+                }
+                sc[i] = (is_v ? c.value_scales : c.key_scales)[row * (DH / 32) + x];
+            }
+        }
+    };
+    auto deliver = [&](int buf, int64_t base) {
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            const int u = tid + i * kThreads;
+            if (kUnits % kThreads && u >= kUnits) continue;
+            const int key = key_of(i), x = u % (DH / 32);
+            const bool is_v = u >= 2 * DH, in = page[i] >= 0 && base + key < end;
+            char* dst = lds + buf * kBuf + (is_v ? kRowsKeys * kStride : 0) + key * kStride;
+            bool odd = false;
+            constexpr uint32_t kExp = DT == FF_BF16 ? 0x7f80u : 0x7c00u;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                uint32_t t[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (STORE == kStoreSame) t[e] = w[i][4 * k + e];
+                    else t[e] = codes2<DT, STORE>(w[i][(4 * k + e) / (STORE == FF_STORE_E4M3 ? 2 : 4)], __uint_as_float(sc[i] << 23), (4 * k + e) % (STORE == FF_STORE_E4M3 ? 2 : 4));
+                    t[e] = in ? t[e] : 0;                            // (what nobody sees may be anything: zeros stand in)
+                    if (is_v && base + kRowsKeys > start) {
+                        // new tokens do not all see each other, and 0 x NaN is NaN: a NaN or infinity among these keys' values stays
+                        // out of the products and is added at the end to the rows that see it
+                        if ((t[e] & kExp) == kExp) t[e] &= 0xffff0000u, odd = true;
+                        if ((t[e] & (kExp << 16)) == (kExp << 16)) t[e] &= 0xffffu, odd = true;
+                    }
+                }
+                *(uint4*)(dst + (STORE == kStoreSame ? k * (DH / 32) + x : 4 * x + k) * 16) = make_uint4(t[0], t[1], t[2], t[3]);
+            }
+            if (odd) s_odd = 1;
+            if (!is_v && x == 0 && (key & 15) == 0) s_have[buf][key >> 4] = page[i] >= 0;
+        }
+    };
+
+    // which of the 16 keys first + 8 (e / 4) + 4 h + e % 4 this lane's row sees (bit e); keys past the end are not asked about
+    const int token_in = min(token, n - 1);
+    const uint8_t* mask = a.mask ? a.mask + (int64_t)b * a.mask_batch + (int64_t)token_in * n : nullptr;
+    auto seen_of = [&](int64_t first) {
+        const int fresh0 = (int)(first - start) + 4 * h;             // (positions fit an int)
+        uint32_t sees = 0;
+        if (mask) {
+            uint32_t byte[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) byte[e] = mask[min(max(fresh0 + 8 * (e >> 2) + (e & 3), 0), n - 1)];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sees |= byte[e] || fresh0 + 8 * (e >> 2) + (e & 3) < 0 ? 1u << e : 0u;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sees |= fresh0 + 8 * (e >> 2) + (e & 3) <= token_in ? 1u << e : 0u;
+        }
+        return sees;
+    };
+
+    const int64_t stride = (int64_t)p.splits * kRowsKeys;
+    int64_t base = (int64_t)split * kRowsKeys;
+    __syncthreads();                           // (s_odd is clear)
+    if (base < end) {
+        look_up(base);
+        fetch(base);
+        look_up(base + stride);
+        deliver(0, base);
+    }
+    __syncthreads();
+    for (int buf = 0; base < end; buf ^= 1, base += stride) {
+        const bool more = base + stride < end;
+        if (more) {
+            fetch(base + stride);
+            look_up(base + 2 * stride);
+        }
+        const uint32_t have = uniform(s_have[buf][0] | s_have[buf][1] << 1 | s_have[buf][2] << 2 | s_have[buf][3] << 3);
+        if (works) {
+            const char* keys = lds + buf * kBuf;
+            const char* values = keys + kRowsKeys * kStride + (4 * h + ((lane & 15) >> 2)) * kStride + (lane & 16) * 2 + (lane & 3) * 8;
+#pragma unroll 1
+            for (int sub = 0; sub < 2; ++sub) {
+                const int64_t first = base + sub * 32;
+                if (first >= end) break;
+                uint4 kf[kSteps];
+                const char* kp = keys + (sub * 32 + col) * kStride + h * 16;
+#pragma unroll
+                for (int x = 0; x < kSteps; ++x) kf[x] = *(const uint4*)(kp + x * 32);
+                f32x16 s;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[e] = 0.f;
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int x = 0; x < kSteps; ++x) s = mma32<DT>(kf[x], qf[x], s);
+                // the values of the same keys, on their way while the weights are made
+                uint2 vf[2][kTiles][2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int y = 0; y < kTiles; ++y) {
+                        const char* vp = values + (sub * 32 + 16 * k) * kStride + y * 64;              // keys 4 h + 0..3 and 8 behind
+                        vf[k][y][0] = read_turned(vp);
+                        vf[k][y][1] = read_turned(vp + 8 * kStride);
+                    }
+                __builtin_amdgcn_sched_barrier(0);
+                float top = kNone;
+                if (((have >> (2 * sub)) & 3u) != 3u || first + 32 > start) {                          // not every row sees every key
+                    uint32_t sees = seen_of(first);
+                    if (!((have >> (2 * sub)) & 1u)) sees &= 0xff00u;
+                    if (!((have >> (2 * sub)) & 2u)) sees &= 0x00ffu;
+                    const int left = (int)(end - first) - 4 * h;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (!((sees >> e) & 1u) || 8 * (e >> 2) + (e & 3) >= left) s[e] = kNone;
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) top = fmaxf(top, s[e]);
+                top *= p.scale2;
+                const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+                top = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+                // (the maximum moves only when a row passes it by 2^8, as in ff_attend.hip)
+                if (__any(top > m + 8.f)) {
+                    const float up = fmaxf(m, top), down = __builtin_amdgcn_exp2f(m - (up == kNone ? 0.f : up));
+                    m = up;
+                    l *= down;
+#pragma unroll
+                    for (int y = 0; y < kTiles; ++y) o[y] *= down;
+                }
+                const float zero = m == kNone ? 0.f : m;
+                float sum = 0.f;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], p.scale2, -zero));
+                    sum += s[e];
+                }
+                l += sum;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint4 pf = make_uint4(pack2<DT>(s[8 * k], s[8 * k + 1]), pack2<DT>(s[8 * k + 2], s[8 * k + 3]),
+                                                pack2<DT>(s[8 * k + 4], s[8 * k + 5]), pack2<DT>(s[8 * k + 6], s[8 * k + 7]));
+#pragma unroll
+                    for (int y = 0; y < kTiles; ++y)
+                        o[y] = mma32<DT>(make_uint4(vf[k][y][0].x, vf[k][y][0].y, vf[k][y][1].x, vf[k][y][1].y), pf, o[y]);
+                }
+            }
+        }
+        if (more) deliver(buf ^ 1, base + stride);
+        __syncthreads();
+    }
+
+    if (!works || row >= p.R) return;
+    if (s_odd) {
+        // rare: the values left out above, to the rows that see them (their weight is positive: infinities and NaN stay what they are)
+        for (int64_t first = ((int64_t)split + max((int64_t)0, start / kRowsKeys - split + p.splits - 1) / p.splits * p.splits) * kRowsKeys; first < end; first += stride) {
+#pragma unroll 1
+            for (int k = 0; k < kRowsKeys; ++k) {
+                const int64_t r = row_of_16(c, p, table, head, first + (k & 48), end);
+                const int64_t fresh = first + k - start;
+                if (r < 0 || first + k >= end) continue;
+                if (fresh >= 0 && !(mask ? mask[fresh] != 0 : fresh <= token)) continue;
+#pragma unroll
+                for (int g = 0; g < DH / 8; ++g) {
+                    float f[4];
+                    fetch4<DT, STORE>(c.values, c.value_scales, r + (k & 15), DH, 2 * g + h, f);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float v = Act<DT>::rnd(f[e]);
+                        if (!(fabsf(v) < __builtin_inff())) o[g >> 2][4 * (g & 3) + e] += v;
+                    }
+                }
+            }
+        }
+    }
+    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+    const float sum = __uint_as_float(both[0]) + __uint_as_float(both[1]);
+    // channel of o[y][e]: 32 y + 8 (e / 4) + 4 h + e % 4
+    if (p.splits > 1) {
+        const int64_t at = (((int64_t)b * kv + head) * p.R + row) * p.splits + split;
+        float* part = p.part + at * DH + 4 * h;
+#pragma unroll
+        for (int y = 0; y < kTiles; ++y)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) *(f32x4*)(part + 32 * y + 8 * g) = f32x4{o[y][4 * g], o[y][4 * g + 1], o[y][4 * g + 2], o[y][4 * g + 3]};
+        if (h == 0) ((float2*)(p.part + p.part_rows * DH))[at] = make_float2(m, sum);
+    } else {
+        char* out = (char*)a.out + ((int64_t)b * a.o_batch + (int64_t)(head * p.G + row - token * p.G) * a.o_head + (int64_t)token * a.o_token) * 2;
+#pragma unroll
+        for (int y = 0; y < kTiles; ++y)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                write_out4<DT>(out, 32 * y + 8 * g + 4 * h, f32x4{o[y][4 * g], o[y][4 * g + 1], o[y][4 * g + 2], o[y][4 * g + 3]}, sum);
+    }
+}
+
+template <int DT, int STORE, int DH, int NW>
+static int launch_rows_nw(const ff_cache_attention_t* a, const AttPlan& p) {
+    constexpr int kBytes = 4 * kRowsKeys * (DH * 2 + 16);
+    static_assert(kBytes + 64 <= 160 * 1024, "two buffers fit the shared memory of a CU");
+    static std::atomic<bool> ready[kMaxDevices];
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= kMaxDevices) dev = -1;
+    if (dev < 0 || !ready[dev].load(std::memory_order_acquire)) {
+        const hipError_t e = hipFuncSetAttribute((const void*)k_cache_attention_rows<DT, STORE, DH, NW>, hipFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+        if (e != hipSuccess) return (int)e;
+        if (dev >= 0) ready[dev].store(true, std::memory_order_release);
+    }
+    const ff_cache_t& c = a->cache;
+    const dim3 grid((uint32_t)p.splits, (uint32_t)(c.kv_heads * p.groups), (uint32_t)c.B);
+    k_cache_attention_rows<DT, STORE, DH, NW><<<grid, 64 * NW, kBytes, (hipStream_t)a->stream>>>(*a, p);
+    return (int)hipGetLastError();
+}
+template <int DT, int STORE, int DH>
+static int launch_rows_dh(const ff_cache_attention_t* a, const AttPlan& p, int waves) {
+    if (waves == 2) return launch_rows_nw<DT, STORE, DH, 2>(a, p);
+    if constexpr (DH < 256)
+        if (waves == 8) return launch_rows_nw<DT, STORE, DH, 8>(a, p);
+    return launch_rows_nw<DT, STORE, DH, 4>(a, p);
+}
+template <int DT, int STORE>
+static int launch_rows_store(const ff_cache_attention_t* a, const AttPlan& p, int waves) {
+    switch (a->cache.dh) {
+        case 32: return launch_rows_dh<DT, STORE, 32>(a, p, waves);
+        case 64: return launch_rows_dh<DT, STORE, 64>(a, p, waves);
+        case 128: return launch_rows_dh<DT, STORE, 128>(a, p, waves);
+        default: return launch_rows_dh<DT, STORE, 256>(a, p, waves);
+    }
+}
+template <int DT> int launch_attention_rows(const ff_cache_attention_t* a, const AttPlan& p, int waves) {
+    if (a->cache.store == FF_STORE_E4M3) return launch_rows_store<DT, FF_STORE_E4M3>(a, p, waves);
+    if (a->cache.store == FF_STORE_E2M1) return launch_rows_store<DT, FF_STORE_E2M1>(a, p, waves);
+    return launch_rows_store<DT, kStoreSame>(a, p, waves);
+}
+template int launch_attention_rows<FF_BF16>(const ff_cache_attention_t*, const AttPlan&, int);
+template int launch_attention_rows<FF_F16>(const ff_cache_attention_t*, const AttPlan&, int);
+
+}  // namespace ff

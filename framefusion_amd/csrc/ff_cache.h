@@ -65,6 +65,18 @@ __device__ inline void fetch8(const void* codes, const uint8_t* scales, int64_t 
     }
 }
 
+// channels [4 u, 4 u + 4), T of 16 bits
+template <int DT, int STORE>
+__device__ inline void fetch4(const void* codes, const uint8_t* scales, int64_t row, int dh, int u, float* f) {
+    const char* p = (const char*)codes + row * row_bytes<DT, STORE>(dh);
+    float x[8];
+    if constexpr (STORE == FF_STORE_E4M3) decode8_e4m3(make_uint2(((const uint32_t*)p)[u], 0), block_scale(scales[row * (dh / 32) + u / 8]), x);
+    else if constexpr (STORE == FF_STORE_E2M1) decode8_e2m1(((const uint16_t*)p)[u], block_scale(scales[row * (dh / 32) + u / 8]), x);
+    else Act<DT>::unpack(make_uint4(((const uint2*)p)[u].x, ((const uint2*)p)[u].y, 0, 0), x);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = x[e];
+}
+
 inline bool cache_aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
 // FF_OK, or what is wrong with the part of a call that names the cache
 int cache_check(const ff_cache_t* c);
