@@ -49,13 +49,15 @@ template <int DT, int STORE> __device__ inline uint32_t codes2(uint32_t w, float
 }
 struct AttPlan {                    // what the host derives once a call
     int G, R, groups;               // heads a kv head, query rows of one (n G), workgroups over the rows
-    int splits, block;              // workgroups over the keys at most; split s takes blocks s, s + splits, .. of so many keys
+    int want, slots, block;         // workgroups over the keys of all sequences: about `want`, at most `slots` = want + B (1: each
+                                    // sequence whole); they take blocks of so many keys
+    int exact;                      // no more than `want`: they fill the chip once, and a second round would cost as much again
     int tiles;                      // many rows: tiles of 32 rows a workgroup
     int page16;                     // page_size / 16 ...
     uint32_t magic;                 // ... and floor(2^32 / page16) (2^32 - 1 for 1)
     float scale2;                   // |scale| log2(e), at least the smallest normal number (0 times a masked score would be NaN)
     uint32_t flip;                  // scale < 0: sign bits of two elements of 16-bit Q, taken up there (fp32: of one)
-    float* part;                    // splits > 1: [B, kv heads, R, splits] x DH sums, then as many (maximum, sum) pairs
+    float* part;                    // slots > 1: [kv heads, R, slots] x DH sums, then as many (maximum, sum) pairs
     int64_t part_rows;
 };
 
@@ -64,11 +66,51 @@ __device__ inline int64_t keys_of(const ff_cache_t& c, int64_t start) {
     const int64_t room = c.n_pages > 0 ? c.table_width * c.page_size : 0;
     return start < 0 ? 0 : min(start + c.n, room);
 }
-// splits that have a block of a sequence of `end` keys (the first one answers for an empty sequence)
-__device__ inline int used_splits(const AttPlan& p, int64_t end) { return (int)max((int64_t)1, min((int64_t)p.splits, (end + p.block - 1) / p.block)); }
+// Which part of the work workgroup `w` over the keys has: split `split` of the `used` ones of sequence `b`, blocks split, split +
+// used, ..; `first` = the slot of the sequence's split 0.  The lengths are on the device alone, so the shares are made there: every
+// wave adds up the blocks of all sequences and deals them out so that each split has about as many (a long sequence gets more
+// splits, an empty one the one that writes its zeros).  All lanes of the wave call it.
+struct Share { int b, split, used, first; };
+// one sequence, or none split: known at once but for `used`, so a kernel's first loads need not wait for the lengths
+__device__ inline bool plain_share(const ff_cache_t& c, const AttPlan& p) { return c.B == 1 || p.slots == 1; }
+__device__ inline int blocks_of(const ff_cache_t& c, const AttPlan& p, int b) { return (int)((keys_of(c, c.start[b]) + p.block - 1) / p.block); }
+__device__ inline bool share_of(const ff_cache_t& c, const AttPlan& p, int w, int of_b, Share& s) {
+    const int B = (int)c.B, lane = threadIdx.x & 63;
+    auto sum = [&](int each) {                    // blocks of all sequences, or with each > 0 their splits of so many
+        int64_t x = 0;
+        for (int b = lane; b < B; b += 64) {
+            const int n = blocks_of(c, p, b);
+            x += each ? max(1, (n + each - 1) / each) : n;
+        }
+#pragma unroll
+        for (int k = 32; k > 0; k >>= 1) x += __shfl_xor(x, k, 64);
+        return x;
+    };
+    const int64_t total = sum(0);
+    int each = (int)max((int64_t)1, (total + p.want - 1) / p.want);
+    if (p.exact && B < p.want) {                  // (shares are rounded up sequence by sequence: where that makes too many, they grow a little)
+        for (int k = 0; k < 6 && sum(each) > p.want; ++k) each += each / 16 + 1;
+    }
+    int before = 0;
+    for (int b0 = 0; b0 < B; b0 += 64) {
+        const int b = b0 + lane, used = b < B ? max(1, (blocks_of(c, p, b) + each - 1) / each) : 0;
+        const int incl = wave_incl_scan_dpp(used);
+        const uint64_t found = of_b < 0 ? __ballot(b < B && before + incl > w) : __ballot(b == of_b);
+        if (found) {
+            const int l = __ffsll((long long)found) - 1;
+            s.b = b0 + l;
+            s.used = __builtin_amdgcn_readlane(used, l);
+            s.first = before + __builtin_amdgcn_readlane(incl, l) - s.used;
+            s.split = of_b < 0 ? w - s.first : 0;
+            return true;
+        }
+        before += __builtin_amdgcn_readlane(incl, 63);
+    }
+    return false;
+}
 
-// the page number (any value) of the 16 keys from `key` on, a multiple of 16, and their first row on it; -1 past the end
-__device__ inline int page_of_16(const AttPlan& p, const int32_t* table, int64_t key, int64_t end, int& off) {
+// the page number (any value) of the 16 keys from `key` on, a multiple of 16, and their first row on it; -1 past the table
+__device__ inline int page_of_16(const ff_cache_t& c, const AttPlan& p, const int32_t* table, int64_t key, int& off) {
     const uint32_t x = (uint32_t)(key >> 4);
     uint32_t slot = __umulhi(x, p.magic);                                      // (one too small at most)
     off = x - slot * p.page16;
@@ -77,7 +119,7 @@ __device__ inline int page_of_16(const AttPlan& p, const int32_t* table, int64_t
         off -= p.page16;
     }
     off *= 16;
-    return key < end ? table[slot] : -1;
+    return key < c.table_width * c.page_size ? table[slot] : -1;
 }
 // row of the cache behind it for one kv head; -1: the keys have no place
 __device__ inline int64_t row_on_page(const ff_cache_t& c, int head, int page, int off) {
@@ -85,8 +127,8 @@ __device__ inline int64_t row_on_page(const ff_cache_t& c, int head, int page, i
 }
 __device__ inline int64_t row_of_16(const ff_cache_t& c, const AttPlan& p, const int32_t* table, int head, int64_t key, int64_t end) {
     int off;
-    const int page = page_of_16(p, table, key, end, off);
-    return row_on_page(c, head, page, off);
+    const int page = page_of_16(c, p, table, key, off);
+    return key < end ? row_on_page(c, head, page, off) : -1;
 }
 
 // four consecutive channels of one output row, sums divided by the weights' total (0: the row saw nothing)
@@ -97,6 +139,6 @@ template <int DT> __device__ inline void write_out4(char* out, int d, f32x4 acc,
 }
 
 // csrc/ff_attend_rows.hip
-template <int DT> int launch_attention_rows(const ff_cache_attention_t* a, const AttPlan& p, int waves);
+template <int DT> int launch_attention_rows(const ff_cache_attention_t* a, const AttPlan& p);
 
 }  // namespace ff

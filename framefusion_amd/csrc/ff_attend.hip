@@ -212,19 +212,28 @@ template <int DT, int STORE, int DH> __device__ inline bool take_out_odd(Raw<DT,
 }
 
 template <int DT, int STORE, int DH, int NT>
-__global__ __launch_bounds__(64 * kAttWaves, DH * NT * (STORE == kStoreSame ? Act<DT>::kBytes : 2) >= 512 ? 1 : 2) void k_cache_attention(const ff_cache_attention_t a, const AttPlan p) {
+__global__ __launch_bounds__(64 * kAttWaves, DH * NT * (STORE == kStoreSame ? Act<DT>::kBytes : 2) > 512 || DH == 256 ? 1 : 2) void k_cache_attention(const ff_cache_attention_t a, const AttPlan p) {
     using G = Geo<DT, STORE, DH>;
     constexpr int kSteps = DH / 32, kTiles = DH / 16, kPad = 4;
     __shared__ float s_o[kAttWaves][16][DH + kPad];
     __shared__ float s_m[kAttWaves][16], s_l[kAttWaves][16];
     const ff_cache_t& c = a.cache;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), q = lane >> 4, col = lane & 15;
-    const int n = (int)c.n, kv = (int)c.kv_heads;
-    const int split = blockIdx.x, b = blockIdx.z, head = blockIdx.y / p.groups, group = blockIdx.y - head * p.groups;
-    const int64_t start = c.start[b];
-    const int64_t end = keys_of(c, start);
-    if (split >= used_splits(p, end)) return;
+    const int n = (int)c.n;
+    const int head = blockIdx.y / p.groups, group = blockIdx.y - head * p.groups;
+    const bool plain = plain_share(c, p);
+    Share share = {p.slots == 1 ? (int)blockIdx.x : 0, p.slots == 1 ? 0 : (int)blockIdx.x, 1, 0};
+    if (!plain && !share_of(c, p, blockIdx.x, -1, share)) return;
+    const int b = share.b, split = share.split;
     const int32_t* table = c.table + (int64_t)b * c.table_width;
+    int page0, page1, off0, off1;
+    auto look_up = [&](int64_t key) {             // the pages of a tile, a tile before its rows are loaded
+        page0 = page_of_16(c, p, table, key, off0);
+        page1 = page_of_16(c, p, table, key + 16, off1);
+    };
+    const int64_t begin = ((int64_t)split * kAttWaves + wave) * kAttTile;
+    look_up(begin);
+    const int64_t start = c.start[b], end = keys_of(c, start);
 
     // the wave's rows of Q, NT tiles of 16; rows past R are zeros
     Frag<DT> qf[NT][kSteps];
@@ -277,23 +286,19 @@ __global__ __launch_bounds__(64 * kAttWaves, DH * NT * (STORE == kStoreSame ? Ac
 
     Raw<DT, STORE, DH> next;
     int64_t next0 = -1, next1 = -1;
-    int page0 = -1, page1 = -1, off0 = 0, off1 = 0;
-    auto look_up = [&](int64_t key) {             // the pages of a tile, a tile before its rows are loaded
-        page0 = page_of_16(p, table, key, end, off0);
-        page1 = page_of_16(p, table, key + 16, end, off1);
-    };
-    auto fetch = [&]() {
-        next0 = row_on_page(c, head, page0, off0);
-        next1 = row_on_page(c, head, page1, off1);
+    auto fetch = [&](int64_t key) {
+        next0 = key < end ? row_on_page(c, head, page0, off0) : -1;
+        next1 = key + 16 < end ? row_on_page(c, head, page1, off1) : -1;
         load_half<DT, STORE, DH>(next, 0, c, next0 < 0 ? 0 : next0, lane);      // (what has no place: any row, left out below)
         load_half<DT, STORE, DH>(next, 1, c, next1 < 0 ? 0 : next1, lane);
     };
     const uint8_t* mask = a.mask ? a.mask + (int64_t)b * a.mask_batch : nullptr;
     bool odd = false;
-    const int64_t begin = ((int64_t)split * kAttWaves + wave) * kAttTile, stride = (int64_t)p.splits * kAttWaves * kAttTile;
+    if (plain && p.slots > 1) share.used = max(1, min(p.want, blocks_of(c, p, b)));
+    if (split >= share.used) return;
+    const int64_t stride = (int64_t)share.used * kAttWaves * kAttTile;
     if (begin < end) {
-        look_up(begin);
-        fetch();
+        fetch(begin);
         look_up(begin + stride);
     }
     for (int64_t base = begin; base < end; base += stride) {
@@ -301,7 +306,7 @@ __global__ __launch_bounds__(64 * kAttWaves, DH * NT * (STORE == kStoreSame ? Ac
         const int64_t row0 = next0, row1 = next1;
         const bool have0 = row0 >= 0, have1 = row1 >= 0;
         if (base + stride < end) {
-            fetch();
+            fetch(base + stride);
             look_up(base + 2 * stride);
         }
         const bool whole = have0 && have1 && base + kAttTile <= start;    // every row sees every key of the tile
@@ -488,8 +493,8 @@ __global__ __launch_bounds__(64 * kAttWaves, DH * NT * (STORE == kStoreSame ? Ac
                 sum += s_l[w][row] * __builtin_amdgcn_exp2f(s_m[w][row] - (most == kNone ? 0.f : most));
                 acc += *(const f32x4*)&s_o[w][row][d];
             }
-            if (p.splits > 1) {
-                const int64_t at = (((int64_t)b * kv + head) * p.R + r) * p.splits + split;
+            if (p.slots > 1) {
+                const int64_t at = ((int64_t)head * p.R + r) * p.slots + blockIdx.x;
                 *(f32x4*)(p.part + at * DH + d) = acc;
                 if (d == 0) ((float2*)(p.part + p.part_rows * DH))[at] = make_float2(most, sum);
             } else {
@@ -501,52 +506,58 @@ __global__ __launch_bounds__(64 * kAttWaves, DH * NT * (STORE == kStoreSame ? Ac
     }
 }
 
-// One workgroup joins the splits of one query row: thread (y, d) sums every kJoin-th split's channel d, the kJoin sums meet in
-// shared memory in fixed order.
+// Joins the splits of query rows, 32 lanes (dh / 4) to a row and kGroup such groups to share its splits: many for the few rows and many
+// splits of single tokens, one where there are rows enough.  The sums meet in fixed order.
 constexpr int kJoinThreads = 256;
-template <int DT, int DH>
+template <int DT, int DH, int kGroup>
 __global__ __launch_bounds__(kJoinThreads) void k_cache_attention_join(const ff_cache_attention_t a, const AttPlan p) {
-    constexpr int kUnits = DH / 4, kJoin = kJoinThreads / kUnits;
-    __shared__ f32x4 s_o[kJoin][kUnits];
-    __shared__ float s_l[kJoin];
-    __shared__ float s_top[kJoinThreads / 64];
+    constexpr int kUnits = DH / 4, kRows = kJoinThreads / kUnits / kGroup;
+    __shared__ f32x4 s_o[kRows * kGroup][kUnits];
+    __shared__ float s_l[kRows * kGroup], s_m[kRows * kGroup];
     const ff_cache_t& c = a.cache;
-    const int r = blockIdx.x, head = blockIdx.y, b = blockIdx.z, kv = (int)c.kv_heads, i = r / p.G;
-    const int used = used_splits(p, keys_of(c, c.start[b]));
-    const int64_t at = (((int64_t)b * kv + head) * p.R + r) * p.splits;
+    const int u = threadIdx.x % kUnits, g = threadIdx.x / kUnits, y = g % kGroup, head = blockIdx.y, b = blockIdx.z;
+    const int r = blockIdx.x * kRows + g / kGroup;
+    Share share = {b, 0, 1, 0};
+    if (c.B == 1) share.used = max(1, min(p.want, blocks_of(c, p, 0)));
+    else share_of(c, p, 0, b, share);
+    const int used = r < p.R ? share.used : 0;
+    const int64_t at = ((int64_t)head * p.R + (r < p.R ? r : 0)) * p.slots + share.first;
     const float2* ml = (const float2*)(p.part + p.part_rows * DH) + at;
-    const int u = threadIdx.x % kUnits, y = threadIdx.x / kUnits;
+    const float* part = p.part + at * DH + u * 4;
     float top = kNone;
-    for (int s = threadIdx.x; s < used; s += kJoinThreads) top = fmaxf(top, ml[s].x);
-#pragma unroll
-    for (int k = 32; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor(top, k, 64));
-    if ((threadIdx.x & 63) == 0) s_top[threadIdx.x >> 6] = top;
-    __syncthreads();
-    top = s_top[0];
-#pragma unroll
-    for (int k = 1; k < kJoinThreads / 64; ++k) top = fmaxf(top, s_top[k]);
+    for (int s = y; s < used; s += kGroup) top = fmaxf(top, ml[s].x);
     const float zero = top == kNone ? 0.f : top;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     float sum = 0.f;
-    for (int s = y; s < used; s += kJoin) {
+#pragma unroll 4
+    for (int s = y; s < used; s += kGroup) {
         const float2 x = ml[s];
         const float w = __builtin_amdgcn_exp2f(x.x - zero);
-        acc += *(const f32x4*)(p.part + (at + s) * DH + u * 4) * w;
+        acc += *(const f32x4*)(part + (int64_t)s * DH) * w;
         sum += x.y * w;
     }
-    s_o[y][u] = acc;
-    if (u == 0) s_l[y] = sum;
-    __syncthreads();
-    if (y == 0) {
-        sum = s_l[0];
+    if constexpr (kGroup > 1) {
+        s_o[g][u] = acc;
+        if (u == 0) s_l[g] = sum, s_m[g] = top;
+        __syncthreads();
+        if (y) return;
+        float most = kNone;
 #pragma unroll
-        for (int k = 1; k < kJoin; ++k) {
-            acc += s_o[k][u];
-            sum += s_l[k];
+        for (int k = 0; k < kGroup; ++k) most = fmaxf(most, s_m[g + k]);
+        const float base = most == kNone ? 0.f : most;
+        acc = f32x4{0.f, 0.f, 0.f, 0.f};
+        sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < kGroup; ++k) {
+            const float w = __builtin_amdgcn_exp2f(s_m[g + k] - base);
+            acc += s_o[g + k][u] * w;
+            sum += s_l[g + k] * w;
         }
-        char* out = (char*)a.out + ((int64_t)b * a.o_batch + (int64_t)(head * p.G + r - i * p.G) * a.o_head + (int64_t)i * a.o_token) * Act<DT>::kBytes;
-        write_out4<DT>(out, u * 4, acc, sum);
     }
+    if (r >= p.R) return;
+    const int i = r / p.G;
+    char* out = (char*)a.out + ((int64_t)b * a.o_batch + (int64_t)(head * p.G + r - i * p.G) * a.o_head + (int64_t)i * a.o_token) * Act<DT>::kBytes;
+    write_out4<DT>(out, u * 4, acc, sum);
 }
 
 static int attention_check(const ff_cache_attention_t* a) {
@@ -555,7 +566,7 @@ static int attention_check(const ff_cache_attention_t* a) {
     if (rc) return rc;
     if (!a->q || !a->out || a->H < 1 || a->H % a->cache.kv_heads || a->mask_batch < 0) return FF_ERR_ARG;
     if (a->cache.dh != 32 && a->cache.dh != 64 && a->cache.dh != 128 && a->cache.dh != 256) return FF_ERR_UNSUPPORTED;
-    if (a->H > 65535 || a->cache.B > 65535 || a->cache.n * a->H > 65535 * 16) return FF_ERR_UNSUPPORTED;
+    if (a->H > 65535 || a->cache.B > 65535 || a->cache.n * a->H > 61439 * 16) return FF_ERR_UNSUPPORTED;      // (grids: kv heads x groups of 16 rows)
     const int64_t per = a->cache.dtype == FF_F32 ? 4 : 8;
     if (!cache_aligned(a->q) || !cache_aligned(a->out)) return FF_ERR_ALIGN;
     const int64_t strides[6] = {a->q_batch, a->q_head, a->q_token, a->o_batch, a->o_head, a->o_token};
@@ -564,12 +575,11 @@ static int attention_check(const ff_cache_attention_t* a) {
     return FF_OK;
 }
 
-// Which kernel serves R query rows, and how many waves share a block of keys.  Up to 32 rows (and fp32, whose products are slow
-// anyway): ff_attend.hip, tiles of 16 rows; more: ff_attend_rows.hip, tiles of 32 rows, a wave each.
-static int row_waves(int dtype, int64_t R, int64_t dh) {
-    if (dtype == FF_F32 || R <= 32) return 0;
-    return R <= 64 ? 2 : R <= 128 || dh == 256 ? 4 : 8;
-}
+// Which kernel serves R query rows, and how many waves share a block of keys there.  Up to 128 rows (and fp32, whose products are
+// slow anyway): 0, ff_attend.hip, whose waves hold 16 or 32 rows and read the cache again for the rows of the next workgroup; more:
+// ff_attend_rows.hip, tiles of 32 rows, a wave each.  4 sequences of 13 474, 28 / 4 heads of 128 in 8 bits: 84 rows 59 us here and 68
+// there, 126 rows 57 and 71, 252 rows 84 and 65.
+static int row_waves(int dtype, int64_t R, int64_t dh) { return dtype == FF_F32 || R <= 128 ? 0 : dh == 256 ? 4 : 8; }
 
 static AttPlan attention_plan(const ff_cache_attention_t* a) {
     const ff_cache_t& c = a->cache;
@@ -593,13 +603,16 @@ static AttPlan attention_plan(const ff_cache_attention_t* a) {
     const double scale2 = a->scale * 1.4426950408889634;
     p.scale2 = fmaxf(fabsf((float)scale2), 1.17549435e-38f);
     p.flip = scale2 < 0 ? (c.dtype == FF_F32 ? 0x80000000u : 0x80008000u) : 0u;
-    const int64_t base = c.B * c.kv_heads * p.groups, room = c.table_width * c.page_size;
-    int64_t s = ((waves ? 2048 / waves : 1024) + base - 1) / base;
-    const int64_t most = (room + p.block - 1) / p.block;
-    s = s < 1 ? 1 : s > 256 ? 256 : s;
-    if (s > most) s = most < 1 ? 1 : most;
-    p.splits = (int)s;
-    p.part_rows = s > 1 ? c.B * c.kv_heads * p.R * s : 0;
+    // workgroups over the keys: enough to fill 256 CUs several times over, no more than there can be blocks; none where every
+    // sequence is one block at most, or where the sequences alone make twice as many workgroups
+    const int64_t base = c.kv_heads * p.groups, blocks = (c.table_width * c.page_size + p.block - 1) / p.block;
+    // (many rows: one workgroup a CU; few rows: two at a time, in two rounds - half or twice as many cost a fifth more)
+    const int64_t fill = waves ? 256 : 1024, want = fill / base > 0 ? fill / base : 1;
+    p.exact = waves != 0;
+    const bool whole = blocks <= 1 || c.B >= 2 * want;
+    p.want = (int)(want < c.B * blocks ? want : c.B * blocks);
+    p.slots = whole ? 1 : (int)(p.want + (c.B > 1 ? c.B : 0));
+    p.part_rows = p.slots > 1 ? c.kv_heads * p.R * p.slots : 0;
     p.part = (float*)a->ws;
     return p;
 }
@@ -607,7 +620,7 @@ static AttPlan attention_plan(const ff_cache_attention_t* a) {
 template <int DT, int STORE, int DH>
 static int launch_attention(const ff_cache_attention_t* a, const AttPlan& p) {
     const ff_cache_t& c = a->cache;
-    const dim3 grid((uint32_t)p.splits, (uint32_t)(c.kv_heads * p.groups), (uint32_t)c.B);
+    const dim3 grid((uint32_t)(p.slots == 1 ? c.B : p.slots), (uint32_t)(c.kv_heads * p.groups));
     hipStream_t st = (hipStream_t)a->stream;
     if constexpr (DH <= (DT == FF_F32 ? 64 : 128))
         if (p.tiles == 2) k_cache_attention<DT, STORE, DH, 2><<<grid, 64 * kAttWaves, 0, st>>>(*a, p);
@@ -623,22 +636,29 @@ static int launch_attention_dh(const ff_cache_attention_t* a, const AttPlan& p) 
         default: return launch_attention<DT, STORE, 256>(a, p);
     }
 }
+template <int DT, int DH, int kGroup>
+static int launch_join_groups(const ff_cache_attention_t* a, const AttPlan& p) {
+    constexpr int kRows = kJoinThreads / (DH / 4) / kGroup;
+    const dim3 grid((uint32_t)((p.R + kRows - 1) / kRows), (uint32_t)a->cache.kv_heads, (uint32_t)a->cache.B);
+    k_cache_attention_join<DT, DH, kGroup><<<grid, kJoinThreads, 0, (hipStream_t)a->stream>>>(*a, p);
+    return (int)hipGetLastError();
+}
 template <int DT, int DH>
 static int launch_join(const ff_cache_attention_t* a, const AttPlan& p) {
-    k_cache_attention_join<DT, DH><<<dim3((uint32_t)p.R, (uint32_t)a->cache.kv_heads, (uint32_t)a->cache.B), kJoinThreads, 0, (hipStream_t)a->stream>>>(*a, p);
-    return (int)hipGetLastError();
+    constexpr int kMost = kJoinThreads / (DH / 4);          // a workgroup a row
+    return a->cache.B * a->cache.kv_heads * p.R >= 1024 ? launch_join_groups<DT, DH, 1>(a, p) : launch_join_groups<DT, DH, kMost>(a, p);
 }
 template <int DT>
 static int launch_attention_t(const ff_cache_attention_t* a, const AttPlan& p) {
     const int waves = row_waves(DT, p.R, a->cache.dh);
-    int rc;
-    if constexpr (DT != FF_F32) rc = waves ? launch_attention_rows<DT>(a, p, waves) : FF_OK;
+    int rc = FF_OK;
+    if constexpr (DT != FF_F32) rc = waves ? launch_attention_rows<DT>(a, p) : FF_OK;
     if (!waves) {
         if (a->cache.store == FF_STORE_E4M3) rc = launch_attention_dh<DT, FF_STORE_E4M3>(a, p);
         else if (a->cache.store == FF_STORE_E2M1) rc = launch_attention_dh<DT, FF_STORE_E2M1>(a, p);
         else rc = launch_attention_dh<DT, kStoreSame>(a, p);
     }
-    if (rc || p.splits == 1) return rc;
+    if (rc || p.slots == 1) return rc;
     switch (a->cache.dh) {
         case 32: return launch_join<DT, 32>(a, p);
         case 64: return launch_join<DT, 64>(a, p);

@@ -432,6 +432,30 @@ def tree(n, B, seed, empty=()):
 def test_attention_types_and_heads(dtype, store, dh):
     attention_case(dtype, store, dh, 2, 4, 1, 32, [77, 0, 31, -1])
     attention_case(dtype, store, dh, 1, 5, 6, 16, [130, 3])
+    attention_case(dtype, store, dh, 1, 5, 40, 16, [130, 3, -1])                            # more rows than one wave or workgroup holds
+    attention_case(dtype, store, dh, 2, 4, 65, 48, [290])
+
+
+def test_attention_of_infinite_values_that_only_some_see():
+    """A value of infinity (its key finite): infinity for the tokens that see it, nothing for the others."""
+    for dtype, n, kv, G in (("bf16", 9, 2, 3), ("bf16", 64, 1, 3), ("fp32", 9, 2, 3)):
+        gen = torch.Generator(device=DEV).manual_seed(n)
+        T = DT[dtype]
+        cache = ffa.new_cache(8, 32, kv, 64, T, None, device=DEV)
+        table, start = torch.arange(8, dtype=torch.int32, device=DEV)[None], torch.tensor([50], dtype=torch.int32, device=DEV)
+        k, v = (torch.randn(1, kv, 50 + n, 64, generator=gen, device=DEV).to(T) for _ in range(2))
+        v[:, :, 52, 3], v[:, :, 55, 3], v[:, :, 55, 9] = math.inf, -math.inf, -math.inf
+        ffa.cache_write(cache, k, v, table, torch.zeros_like(start))
+        q = torch.randn(1, kv * G, n, 64, generator=gen, device=DEV).to(T)
+        got = ffa.cache_attention(q, cache, table, start, mask=torch.eye(n, dtype=torch.bool, device=DEV))
+        odd = torch.zeros(n, 64, dtype=torch.bool, device=DEV)
+        odd[2, 3] = odd[5, 3] = odd[5, 9] = True
+        assert (got[0, :, 2, 3] == math.inf).all() and (got[0, :, 5, 3] == -math.inf).all() and (got[0, :, 5, 9] == -math.inf).all()
+        assert torch.isfinite(got[0][:, ~odd]).all()
+        causal = ffa.cache_attention(q, cache, table, start)
+        assert torch.isfinite(causal[0, :, :2]).all() and (causal[0, :, 2:5, 3] == math.inf).all() and torch.isnan(causal[0, :, 5:, 3]).all()
+        assert (causal[0, :, 5:, 9] == -math.inf).all() and torch.isfinite(causal[0][:, :, 10:]).all()
+
 
 
 @pytest.mark.parametrize("store", [None, "fp8", "fp4"])
