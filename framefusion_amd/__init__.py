@@ -11,7 +11,8 @@ from .utils import get_attr_by_name, scaled_dot_product_attention, last_query_im
 from ._lib import FrameFusionHipError, build, load  # noqa: F401
 from .pair import FrameFusionPair  # noqa: F401
 from .rotary import rotary_frequencies, rotary_tables, apply_rotary  # noqa: F401
-from .cache import (CacheTensors, new_cache, cache_write, cache_read, cache_keep, cache_attention)  # noqa: F401
+from .cache import (CacheTensors, new_cache, cache_write, cache_read, cache_keep, cache_attention,
+                    ReducedCache)  # noqa: F401
 from . import layout, baseline  # noqa: F401
 
 __all__ = ["FrameFusion", "apply_framefusion", "get_token_type", "replace_framefusion_forward",
@@ -19,4 +20,4 @@ __all__ = ["FrameFusion", "apply_framefusion", "get_token_type", "replace_framef
            "get_attr_by_name", "cosine_similarity", "find_contigious_latter_index", "call_b_with_residual",
            "TEXT_TOKEN", "IGNORE_TOKEN", "FrameFusionPair", "FrameFusionHipError", "build", "load", "layout", "baseline",
            "rotary_frequencies", "rotary_tables", "apply_rotary", "CacheTensors", "new_cache", "cache_write", "cache_read",
-           "cache_keep", "cache_attention"]
+           "cache_keep", "cache_attention", "ReducedCache"]

@@ -208,3 +208,106 @@ def cache_attention(query: torch.Tensor, cache, table: torch.Tensor, start: torc
         if rc:
             _lib.check(rc, "ff_cache_attention")
     return out.transpose(1, 2)
+
+
+class ReducedCache:
+    """The keys and values of one sequence behind a reduced prefill: another length in every layer, all layers in one pool of pages.
+
+    Passed as ``past_key_values`` to a Qwen2 / Qwen2-VL model patched by ``apply_framefusion`` it takes the place of transformers'
+    DynamicCache: the prefill writes each layer's (rotated, reduced) keys and values once, in 16, 8 or 4 bits, and every later call
+    runs ``cache_attention`` over them.  A call with ``tree_mask`` (bool [n, n]) attends as a tree of drafted tokens and leaves them
+    pending until ``keep(accepted)``.
+
+    ``max_tokens`` bounds the length of every layer; ``pages`` the pool (default: enough for ``max_tokens`` everywhere - a reduced
+    prefill needs far fewer).  One instance serves one stream of calls, like the reference's module."""
+
+    def __init__(self, layers: int, kv_heads: int, head_dim: int, max_tokens: int, dtype: torch.dtype = torch.bfloat16,
+                 store: Optional[str] = None, page_size: int = 64, pages: Optional[int] = None, device="cuda"):
+        if layers < 1 or max_tokens < 1:
+            raise FrameFusionHipError("ReducedCache: layers and max_tokens must be positive")
+        width = -(-max_tokens // page_size) if page_size > 0 else 0
+        self.tensors = new_cache(layers * width if pages is None else pages, page_size, kv_heads, head_dim, dtype, store, device)
+        self.dtype, self.page_size, self.max_tokens = dtype, page_size, max_tokens
+        self.lengths = [0] * layers                 # tokens held, without pending ones
+        self.pending = [0] * layers                 # tokens written behind them by the current step
+        self._pages = [[] for _ in range(layers)]
+        self._free = list(range(self.tensors.keys.shape[0] - 1, -1, -1))
+        dev = self.tensors.keys.device
+        self._table = torch.full((layers, width), -1, dtype=torch.int32, device=dev)
+        self._start = torch.zeros(layers, dtype=torch.int32, device=dev)
+        self._rows = [(self._table[i:i + 1], self._start[i:i + 1]) for i in range(layers)]
+
+    def get_seq_length(self, layer_idx: int = 0) -> int:
+        return self.lengths[layer_idx]
+
+    def __len__(self) -> int:
+        return len(self.lengths)
+
+    def _room(self, layer, count):
+        """Pages for `count` tokens of a layer."""
+        if count > self.max_tokens:
+            raise FrameFusionHipError(f"ReducedCache: {count} tokens in layer {layer}, max_tokens is {self.max_tokens}")
+        have = self._pages[layer]
+        more = -(-count // self.page_size) - len(have)
+        if more > 0:
+            if more > len(self._free):
+                raise FrameFusionHipError(f"ReducedCache: layer {layer} needs {more} more pages, {len(self._free)} of {self.tensors.keys.shape[0]} are free")
+            new = [self._free.pop() for _ in range(more)]
+            self._table[layer, len(have):len(have) + more] = torch.tensor(new, dtype=torch.int32)
+            have += new
+
+    def append(self, layer: int, key: torch.Tensor, value: torch.Tensor) -> None:
+        """Writes key and value [1, kv_heads, n, head_dim] behind the layer's tokens; they count once ``advance`` or ``keep`` is called."""
+        if key.ndim != 4 or key.shape[0] != 1:
+            raise FrameFusionHipError(f"ReducedCache: one sequence, keys [1, kv_heads, n, head_dim], got {tuple(key.shape)}")
+        if self.pending[layer]:
+            raise FrameFusionHipError("ReducedCache: tokens of the last step are pending; call advance() or keep() first")
+        self._room(layer, self.lengths[layer] + key.shape[2])
+        cache_write(self.tensors, key, value, *self._rows[layer])
+        self.pending[layer] = key.shape[2]
+
+    def attend(self, layer: int, query: torch.Tensor, mask: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
+        """``cache_attention`` of the layer's pending tokens."""
+        if query.ndim != 4 or query.shape[2] != self.pending[layer]:
+            raise FrameFusionHipError(f"ReducedCache: {self.pending[layer]} tokens are pending in layer {layer}, query is {tuple(query.shape)}")
+        return cache_attention(query, self.tensors, *self._rows[layer], mask=mask, scale=scale)
+
+    def _count(self, added):
+        """The pending tokens of every layer become `added` held ones."""
+        self.lengths = [n + a for n, a in zip(self.lengths, added)]
+        self.pending = [0] * len(added)
+        if min(added) == max(added):
+            if added[0]:
+                self._start += added[0]
+        else:
+            self._start.copy_(torch.tensor(self.lengths, dtype=torch.int32))
+
+    def advance(self) -> None:
+        """Every pending token counts from now on."""
+        self._count(self.pending)
+
+    def keep(self, accepted) -> None:
+        """Of the pending drafted tokens the ``accepted`` ones (increasing indices, the same in every layer) stay, in one launch for all
+        layers; the others are forgotten."""
+        accepted = [int(x) for x in accepted]
+        n = self.pending[0]
+        if min(self.pending) != max(self.pending) or any(a >= b for a, b in zip(accepted, accepted[1:])) \
+                or (accepted and not 0 <= accepted[0] <= accepted[-1] < n):
+            raise FrameFusionHipError(f"ReducedCache: accepted must be increasing indices of the {n} pending tokens, got {accepted}")
+        if accepted and accepted != list(range(len(accepted))):
+            lists = torch.tensor(accepted, dtype=torch.int32, device=self._table.device).expand(len(self.lengths), -1).contiguous()
+            cache_keep(self.tensors, self._table, self._start, lists)
+        self._count([len(accepted)] * len(self.lengths))
+
+    def dense(self, layer: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The layer's keys and values [1, kv_heads, length, head_dim], read back."""
+        return cache_read(self.tensors, self._rows[layer][0], torch.zeros_like(self._rows[layer][1]), self.lengths[layer], dtype=self.dtype)
+
+    def reset(self) -> None:
+        """Empty again; every page is free."""
+        for have in self._pages:
+            self._free += have
+            have.clear()
+        self._table.fill_(-1)
+        self._start.zero_()
+        self.lengths, self.pending = [0] * len(self.lengths), [0] * len(self.lengths)

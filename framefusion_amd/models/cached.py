@@ -1,0 +1,49 @@
+"""What the Qwen2 and Qwen2-VL adapters do differently with a ``ReducedCache``: rotation, cache and decoding attention by this
+package's kernels.  The prefill's own attention (and the importance hook) stay as they are; its keys and values are written to the cache
+as they come, reduced, one layer shorter than the one before."""
+from __future__ import annotations
+
+from ..cache import ReducedCache
+from ..rotary import apply_rotary, rotary_tables
+
+
+def continues(past_key_values, layer_idx) -> bool:
+    """Whether a layer's call is a step behind a prefill (nothing is reduced then)."""
+    return isinstance(past_key_values, ReducedCache) and past_key_values.get_seq_length(layer_idx) > 0
+
+
+def position_tables(model, cache, hidden_states, position_ids, attention_mask, tree_mask):
+    """[cos, sin] of the step's positions, formed in 64 bits from the model's own frequencies."""
+    if attention_mask is not None:
+        raise NotImplementedError("a ReducedCache serves one unpadded sequence: run with attention_mask=None (drafted trees: tree_mask)")
+    if hidden_states.shape[0] != 1:
+        raise NotImplementedError("a ReducedCache serves one sequence (FrameFusion reduces one sample a prefill)")
+    if any(cache.pending):
+        raise RuntimeError("drafted tokens are pending: call cache.keep(accepted) before the next step")
+    if tree_mask is not None and not cache.get_seq_length():
+        raise ValueError("tree_mask needs a prefilled cache")
+    rotary = model.rotary_emb
+    if getattr(rotary, "rope_type", "default") in ("dynamic", "longrope"):      # (frequencies that follow the length)
+        return list(rotary(hidden_states, position_ids))
+    return list(rotary_tables(position_ids.contiguous(), rotary.inv_freq.double(), dtype=hidden_states.dtype, factor=rotary.attention_scaling))
+
+
+def rotate(query_states, key_states, cos, sin, sections=None):
+    return apply_rotary(query_states, key_states, cos, sin, sections=sections)
+
+
+def cached_attention(attention, cache, query_states, key_states, value_states, attention_mask, tree_mask):
+    """Writes the step's keys and values; the attention output [1, n, H, dh] of a step behind a prefill, None for a prefill."""
+    step = cache.get_seq_length(attention.layer_idx) > 0
+    if step and (attention_mask is not None or getattr(attention, "sliding_window", None) is not None):
+        raise NotImplementedError("a step over a ReducedCache takes neither an attention_mask nor a sliding window")
+    cache.append(attention.layer_idx, key_states, value_states)
+    if not step:
+        return None
+    return cache.attend(attention.layer_idx, query_states, mask=tree_mask, scale=attention.scaling).transpose(1, 2)
+
+
+def finish_step(cache, tree_mask) -> None:
+    """A step's tokens count at its end; drafted ones wait for ``cache.keep``."""
+    if isinstance(cache, ReducedCache) and tree_mask is None:
+        cache.advance()

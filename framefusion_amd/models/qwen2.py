@@ -12,17 +12,22 @@ Same protocol as the reference's ``framefusion/models/qwen2/modeling_qwen2.py``:
 
 The multimodal packer that builds ``patch_type`` lives outside the LLM (llava_video.py:321-338);
 callers invoke ``model.framefusion.prepare(...)`` themselves before the prefill.
+
+With a ``ReducedCache`` as ``past_key_values`` the layers rotate with ``apply_rotary`` and decode through ``cache_attention``
+(models/cached.py); any other cache takes the path above, unchanged.
 """
 from __future__ import annotations
 
 import torch
 
+from ..cache import ReducedCache
 from ..interface import Family, register_family
 from ..main import call_b_with_residual
 from ..utils import last_query_importance
+from .cached import cached_attention, continues, finish_step, position_tables, rotate
 
 
-def qwen2_attention_forward(self, hidden_states, position_embeddings, attention_mask, past_key_values=None, **kwargs):
+def qwen2_attention_forward(self, hidden_states, position_embeddings, attention_mask, past_key_values=None, tree_mask=None, **kwargs):
     from transformers.models.qwen2.modeling_qwen2 import (ALL_ATTENTION_FUNCTIONS, apply_rotary_pos_emb,
                                                            eager_attention_forward)
     input_shape = hidden_states.shape[:-1]
@@ -31,9 +36,15 @@ def qwen2_attention_forward(self, hidden_states, position_embeddings, attention_
     key_states = self.k_proj(hidden_states).view(hidden_shape).transpose(1, 2)
     value_states = self.v_proj(hidden_states).view(hidden_shape).transpose(1, 2)
     cos, sin = position_embeddings
-    query_states, key_states = apply_rotary_pos_emb(query_states, key_states, cos, sin)
-    if past_key_values is not None:
-        key_states, value_states = past_key_values.update(key_states, value_states, self.layer_idx)
+    if isinstance(past_key_values, ReducedCache):
+        query_states, key_states = rotate(query_states, key_states, cos, sin)
+        attn_output = cached_attention(self, past_key_values, query_states, key_states, value_states, attention_mask, tree_mask)
+        if attn_output is not None:
+            return self.o_proj(attn_output.reshape(*input_shape, -1)), None
+    else:
+        query_states, key_states = apply_rotary_pos_emb(query_states, key_states, cos, sin)
+        if past_key_values is not None:
+            key_states, value_states = past_key_values.update(key_states, value_states, self.layer_idx)
 
     importance = None
     q_len = query_states.shape[2]
@@ -52,7 +63,8 @@ def qwen2_attention_forward(self, hidden_states, position_embeddings, attention_
 
 def qwen2_decoder_forward(self, hidden_states, attention_mask=None, position_ids=None, past_key_values=None,
                           use_cache=False, position_embeddings=None, **kwargs):
-    if self.self_attn.layer_idx == 0:                                        # modeling_qwen2.py:45-46
+    reducing = not continues(past_key_values, self.self_attn.layer_idx)
+    if self.self_attn.layer_idx == 0 and reducing:                           # modeling_qwen2.py:45-46
         hidden_states, position_embeddings, attention_mask = self.framefusion(
             hidden_states, position_embeddings, attention_mask)
     residual = hidden_states
@@ -62,8 +74,11 @@ def qwen2_decoder_forward(self, hidden_states, attention_mask=None, position_ids
                                                use_cache=use_cache, position_embeddings=position_embeddings, **kwargs)
     # modeling_qwen2.py:64-67: hidden = residual + attention output, then call B - here the add is formed
     # inside the reduction's two streaming passes (a plain add when no reduction is due)
-    hidden_states, position_embeddings, attention_mask = call_b_with_residual(
-        self.framefusion, residual, hidden_states, position_embeddings, attention_mask, importance)
+    if reducing:
+        hidden_states, position_embeddings, attention_mask = call_b_with_residual(
+            self.framefusion, residual, hidden_states, position_embeddings, attention_mask, importance)
+    else:
+        hidden_states = residual + hidden_states
     residual = hidden_states
     hidden_states = self.mlp(self.post_attention_layernorm(hidden_states))
     hidden_states = residual + hidden_states
@@ -84,10 +99,15 @@ def qwen2_model_forward(self, input_ids=None, attention_mask=None, position_ids=
     if position_ids is None:
         seen = past_key_values.get_seq_length() if past_key_values is not None else 0
         position_ids = (torch.arange(inputs_embeds.shape[1], device=inputs_embeds.device) + seen).unsqueeze(0)
-    causal_mask = create_causal_mask(config=self.config, inputs_embeds=inputs_embeds, attention_mask=attention_mask,
-                                     past_key_values=past_key_values, position_ids=position_ids)
     hidden_states = inputs_embeds
-    position_embeddings = list(self.rotary_emb(hidden_states, position_ids))  # modeling_qwen2.py:263-266
+    if isinstance(past_key_values, ReducedCache):
+        causal_mask = None
+        position_embeddings = position_tables(self, past_key_values, hidden_states, position_ids, attention_mask,
+                                              kwargs.get("tree_mask"))
+    else:
+        causal_mask = create_causal_mask(config=self.config, inputs_embeds=inputs_embeds, attention_mask=attention_mask,
+                                         past_key_values=past_key_values, position_ids=position_ids)
+        position_embeddings = list(self.rotary_emb(hidden_states, position_ids))  # modeling_qwen2.py:263-266
     lengths = []
     for decoder_layer in self.layers[: self.config.num_hidden_layers]:
         hidden_states, position_embeddings, causal_mask = decoder_layer(      # modeling_qwen2.py:304-305
@@ -95,6 +115,7 @@ def qwen2_model_forward(self, input_ids=None, attention_mask=None, position_ids=
             position_ids=position_ids, past_key_values=past_key_values, use_cache=use_cache, **kwargs)
         lengths.append(hidden_states.shape[1])
     self.framefusion_lengths = lengths
+    finish_step(past_key_values, kwargs.get("tree_mask"))
     hidden_states = self.norm(hidden_states)
     return BaseModelOutputWithPast(last_hidden_state=hidden_states,
                                    past_key_values=past_key_values if use_cache else None)

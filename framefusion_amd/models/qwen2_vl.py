@@ -11,20 +11,25 @@ pre-hook on transformers' ``Qwen2VLModel`` (the module that owns the vision towe
 ``input_ids`` + ``video_grid_thw``): on a prefill with a video it derives the layout with
 ``framefusion_amd.layout.qwen2_vl_layout`` and calls ``framefusion.prepare``.  Bare text-decoder
 wrappers have no such inputs: their callers invoke ``model.framefusion.prepare(...)`` themselves.
+
+With a ``ReducedCache`` as ``past_key_values`` the layers rotate with ``apply_rotary`` and decode through ``cache_attention``
+(models/cached.py); any other cache takes the path above, unchanged.
 """
 from __future__ import annotations
 
 import torch
 
+from ..cache import ReducedCache
 from ..interface import Family, register_family
 from ..main import call_b_with_residual
 from ..utils import last_query_importance
+from .cached import cached_attention, continues, finish_step, position_tables, rotate
 
 NUM_IMPORTANCE_QUERIES = 4           # modeling_qwen2_vl.py:296
 
 
 def qwen2vl_attention_forward(self, hidden_states, attention_mask=None, position_ids=None, past_key_values=None,
-                              output_attentions=False, use_cache=False, position_embeddings=None, **kwargs):
+                              output_attentions=False, use_cache=False, position_embeddings=None, tree_mask=None, **kwargs):
     from transformers.models.qwen2_vl.modeling_qwen2_vl import (ALL_ATTENTION_FUNCTIONS, apply_multimodal_rotary_pos_emb,
                                                                  eager_attention_forward)
     bsz, q_len, _ = hidden_states.size()
@@ -32,10 +37,16 @@ def qwen2vl_attention_forward(self, hidden_states, attention_mask=None, position
     key_states = self.k_proj(hidden_states).view(bsz, q_len, -1, self.head_dim).transpose(1, 2)
     value_states = self.v_proj(hidden_states).view(bsz, q_len, -1, self.head_dim).transpose(1, 2)
     cos, sin = position_embeddings
-    query_states, key_states = apply_multimodal_rotary_pos_emb(query_states, key_states, cos, sin,
-                                                               self.config.rope_parameters["mrope_section"])
-    if past_key_values is not None:
-        key_states, value_states = past_key_values.update(key_states, value_states, self.layer_idx)
+    sections = self.config.rope_parameters["mrope_section"]
+    if isinstance(past_key_values, ReducedCache):
+        query_states, key_states = rotate(query_states, key_states, cos, sin, sections)
+        attn_output = cached_attention(self, past_key_values, query_states, key_states, value_states, attention_mask, tree_mask)
+        if attn_output is not None:
+            return self.o_proj(attn_output.reshape(bsz, q_len, -1)), None
+    else:
+        query_states, key_states = apply_multimodal_rotary_pos_emb(query_states, key_states, cos, sin, sections)
+        if past_key_values is not None:
+            key_states, value_states = past_key_values.update(key_states, value_states, self.layer_idx)
 
     importance = None
     ff = self.framefusion
@@ -54,7 +65,8 @@ def qwen2vl_attention_forward(self, hidden_states, attention_mask=None, position
 
 def qwen2vl_decoder_forward(self, hidden_states, attention_mask=None, position_ids=None, past_key_values=None,
                             use_cache=False, position_embeddings=None, **kwargs):
-    if self.self_attn.layer_idx == 0:                                        # modeling_qwen2_vl.py:178-179
+    reducing = not continues(past_key_values, self.self_attn.layer_idx)
+    if self.self_attn.layer_idx == 0 and reducing:                           # modeling_qwen2_vl.py:178-179
         hidden_states, position_embeddings, attention_mask = self.framefusion(
             hidden_states, position_embeddings, attention_mask)
     residual = hidden_states
@@ -62,8 +74,11 @@ def qwen2vl_decoder_forward(self, hidden_states, attention_mask=None, position_i
     hidden_states, importance = self.self_attn(hidden_states=hidden_states, attention_mask=attention_mask,
                                                position_ids=position_ids, past_key_values=past_key_values,
                                                use_cache=use_cache, position_embeddings=position_embeddings, **kwargs)
-    hidden_states, position_embeddings, attention_mask = call_b_with_residual(    # modeling_qwen2_vl.py:197-200
-        self.framefusion, residual, hidden_states, position_embeddings, attention_mask, importance)
+    if reducing:
+        hidden_states, position_embeddings, attention_mask = call_b_with_residual(    # modeling_qwen2_vl.py:197-200
+            self.framefusion, residual, hidden_states, position_embeddings, attention_mask, importance)
+    else:
+        hidden_states = residual + hidden_states
     residual = hidden_states
     hidden_states = self.mlp(self.post_attention_layernorm(hidden_states))
     hidden_states = residual + hidden_states
@@ -90,10 +105,15 @@ def qwen2vl_text_model_forward(self, input_ids=None, attention_mask=None, positi
     text_position_ids = None
     if position_ids.ndim == 3 and position_ids.shape[0] == 4:
         text_position_ids, position_ids = position_ids[0], position_ids[1:]
-    causal_mask = create_causal_mask(config=self.config, inputs_embeds=inputs_embeds, attention_mask=attention_mask,
-                                     past_key_values=past_key_values, position_ids=text_position_ids)
     hidden_states = inputs_embeds
-    position_embeddings = list(self.rotary_emb(hidden_states, position_ids))  # [cos, sin], each [3, 1, L, dh]
+    if isinstance(past_key_values, ReducedCache):
+        causal_mask = None
+        position_embeddings = position_tables(self, past_key_values, hidden_states, position_ids, attention_mask,
+                                              kwargs.get("tree_mask"))
+    else:
+        causal_mask = create_causal_mask(config=self.config, inputs_embeds=inputs_embeds, attention_mask=attention_mask,
+                                         past_key_values=past_key_values, position_ids=text_position_ids)
+        position_embeddings = list(self.rotary_emb(hidden_states, position_ids))  # [cos, sin], each [3, 1, L, dh]
     lengths = []
     for decoder_layer in self.layers:
         hidden_states, position_embeddings, causal_mask = decoder_layer(
@@ -101,6 +121,7 @@ def qwen2vl_text_model_forward(self, input_ids=None, attention_mask=None, positi
             position_ids=None, past_key_values=past_key_values, use_cache=use_cache, **kwargs)
         lengths.append(hidden_states.shape[1])
     self.framefusion_lengths = lengths
+    finish_step(past_key_values, kwargs.get("tree_mask"))
     hidden_states = self.norm(hidden_states)
     return BaseModelOutputWithPast(last_hidden_state=hidden_states, past_key_values=past_key_values)
 
