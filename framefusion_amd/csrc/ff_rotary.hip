@@ -3,28 +3,6 @@
 
 namespace ff {
 
-// One thread an angle.  position * inv_freq is formed in turns in fp64 (2^-52 of up to 2^31 turns: 2^-21 of a turn at the far
-// end, 2^-31 at a million), its whole turns are taken off there, and only the rest goes to fp32.
-template <int DT>
-__global__ __launch_bounds__(256) void k_rotary_tables(const int64_t* __restrict__ positions, int64_t total, const double* __restrict__ inv_freq,
-                                                       int half, float factor, int interleaved, void* __restrict__ cos_out, void* __restrict__ sin_out) {
-    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (at >= total) return;
-    const int64_t p = at / half;
-    const int i = (int)(at - p * half);
-    const double turns = (double)positions[p] * (inv_freq[i] * 0.15915494309189533577);
-    const float rest = (float)(turns - rint(turns));
-    float s, c;
-    sincospif(2.f * rest, &s, &c);
-    c *= factor;
-    s *= factor;
-    const int64_t first = p * 2 * half + (interleaved ? 2 * i : i), second = interleaved ? first + 1 : first + half;
-    Act<DT>::store1(cos_out, first, c);
-    Act<DT>::store1(cos_out, second, c);
-    Act<DT>::store1(sin_out, first, s);
-    Act<DT>::store1(sin_out, second, s);
-}
-
 // kVec consecutive channels as floats
 template <int DT, int kVec> __device__ inline void get(const void* p, int64_t at, float* f) {
     if constexpr (kVec == 1) {
@@ -47,6 +25,46 @@ template <int DT, int kVec> __device__ inline void put(void* p, int64_t at, floa
             float* x = f + k * Act<DT>::kPer16;
             if constexpr (DT == FF_BF16) w[k] = Act<DT>::pack_rne(x);
             else w[k] = Act<DT>::pack(x);
+        }
+    }
+}
+
+// kVec consecutive angles of one position to a thread, blockDim.x threads to a position.  position * inv_freq is formed in turns in
+// fp64 (2^-52 of up to 2^31 turns: 2^-21 of a turn at the far end, 2^-31 at a million), its whole turns are taken off there, and only
+// the rest goes to fp32.  The tables are written in 16-byte pieces (one element at a time where half a row does not allow it): with
+// two bytes a thread and a 64-bit division to find the position the stores and the division cost as much again as the bytes.
+template <int DT, int kVec>
+__global__ __launch_bounds__(256) void k_rotary_tables(const int64_t* __restrict__ positions, int64_t n, const double* __restrict__ inv_freq,
+                                                       int half, float factor, int interleaved, void* __restrict__ cos_out, void* __restrict__ sin_out) {
+    const int64_t p = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    if (p >= n) return;
+    const double position = (double)positions[p];
+    for (int i = threadIdx.x * kVec; i < half; i += blockDim.x * kVec) {
+        float c[kVec], s[kVec];
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+            const double turns = position * (inv_freq[i + e] * 0.15915494309189533577);
+            sincospif(2.f * (float)(turns - rint(turns)), &s[e], &c[e]);
+            c[e] *= factor;
+            s[e] *= factor;
+        }
+        const int64_t row = p * 2 * half;
+        if (interleaved) {
+            float cc[2 * kVec], ss[2 * kVec];
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) {
+                cc[2 * e] = cc[2 * e + 1] = c[e];
+                ss[2 * e] = ss[2 * e + 1] = s[e];
+            }
+            put<DT, kVec>(cos_out, row + 2 * i, cc);
+            put<DT, kVec>(cos_out, row + 2 * i + kVec, cc + kVec);
+            put<DT, kVec>(sin_out, row + 2 * i, ss);
+            put<DT, kVec>(sin_out, row + 2 * i + kVec, ss + kVec);
+        } else {
+            put<DT, kVec>(cos_out, row + i, c);
+            put<DT, kVec>(cos_out, row + half + i, c);
+            put<DT, kVec>(sin_out, row + i, s);
+            put<DT, kVec>(sin_out, row + half + i, s);
         }
     }
 }
@@ -122,6 +140,18 @@ __global__ __launch_bounds__(256) void k_rotary_apply(const ff_rotary_t a) {
 
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
+template <int DT>
+static int launch_tables(const int64_t* positions, int64_t n, const double* inv_freq, int half, float factor, int interleaved, void* cos, void* sin,
+                         hipStream_t st) {
+    constexpr int kVec = Act<DT>::kPer16;
+    const bool wide = half % kVec == 0 && aligned16(cos) && aligned16(sin);
+    const int units = wide ? half / kVec : half, x = min(units, 256), y = 256 / x;
+    const dim3 block(x, y), grid((uint32_t)((n + y - 1) / y));
+    if (wide) k_rotary_tables<DT, kVec><<<grid, block, 0, st>>>(positions, n, inv_freq, half, factor, interleaved, cos, sin);
+    else k_rotary_tables<DT, 1><<<grid, block, 0, st>>>(positions, n, inv_freq, half, factor, interleaved, cos, sin);
+    return (int)hipGetLastError();
+}
+
 template <int DT, int TDT, int kVec>
 static int launch_apply(const ff_rotary_t* a) {
     const int units = (int)(a->rot / 2 / kVec + (a->dh - a->rot) / kVec), x = min(units, 256);
@@ -155,15 +185,12 @@ extern "C" int ff_rotary_tables(const int64_t* positions, int64_t n, const doubl
                                 int dtype, void* cos, void* sin, ff_stream_t stream) {
     if (n < 0 || half < 1 || !positions || !inv_freq || !cos || !sin) return FF_ERR_ARG;
     if (dtype != FF_F32 && dtype != FF_BF16 && dtype != FF_F16) return FF_ERR_ARG;
-    if (half > 4096 || n > (int64_t)0x7fffffff * 256 / half) return FF_ERR_UNSUPPORTED;
+    if (half > 4096 || n > 0x7fffffff) return FF_ERR_UNSUPPORTED;
     if (n == 0) return FF_OK;
-    const int64_t total = n * half;
-    const uint32_t grid = (uint32_t)((total + 255) / 256);
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == FF_F32) ff::k_rotary_tables<FF_F32><<<grid, 256, 0, st>>>(positions, total, inv_freq, (int)half, (float)factor, interleaved, cos, sin);
-    else if (dtype == FF_BF16) ff::k_rotary_tables<FF_BF16><<<grid, 256, 0, st>>>(positions, total, inv_freq, (int)half, (float)factor, interleaved, cos, sin);
-    else ff::k_rotary_tables<FF_F16><<<grid, 256, 0, st>>>(positions, total, inv_freq, (int)half, (float)factor, interleaved, cos, sin);
-    return (int)hipGetLastError();
+    if (dtype == FF_F32) return ff::launch_tables<FF_F32>(positions, n, inv_freq, (int)half, (float)factor, interleaved, cos, sin, st);
+    if (dtype == FF_BF16) return ff::launch_tables<FF_BF16>(positions, n, inv_freq, (int)half, (float)factor, interleaved, cos, sin, st);
+    return ff::launch_tables<FF_F16>(positions, n, inv_freq, (int)half, (float)factor, interleaved, cos, sin, st);
 }
 
 extern "C" int ff_rotary_apply(const ff_rotary_t* a) {

@@ -44,6 +44,8 @@ def qwen2vl_attention_forward(self, hidden_states, attention_mask=None, position
         if attn_output is not None:
             return self.o_proj(attn_output.reshape(bsz, q_len, -1)), None
     else:
+        if tree_mask is not None:
+            raise ValueError("tree_mask needs a ReducedCache")
         query_states, key_states = apply_multimodal_rotary_pos_emb(query_states, key_states, cos, sin, sections)
         if past_key_values is not None:
             key_states, value_states = past_key_values.update(key_states, value_states, self.layer_idx)

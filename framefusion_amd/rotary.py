@@ -13,7 +13,10 @@ import torch
 from . import _lib
 from ._lib import FrameFusionHipError
 
-_get_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_get_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
+_CODE = _lib.DTYPE_CODE
 
 
 def rotary_frequencies(dim: int, base: float = 10000.0, scaling: Optional[dict] = None) -> Tuple[torch.Tensor, float]:
@@ -75,7 +78,7 @@ def rotary_tables(positions: torch.Tensor, inv_freq: torch.Tensor, dtype: torch.
     dev = positions.device
     if positions.dtype != torch.int64 or inv_freq.dtype != torch.float64 or inv_freq.ndim != 1 or inv_freq.device != dev:
         raise FrameFusionHipError("rotary_tables: positions must be int64, inv_freq a float64 vector on the same device")
-    code = _lib.DTYPE_CODE.get(dtype)
+    code = _CODE.get(dtype)
     if code is None:
         raise FrameFusionHipError(f"rotary_tables: dtype {dtype} is not float32, bfloat16 or float16")
     if positions.requires_grad or inv_freq.requires_grad:
@@ -87,8 +90,8 @@ def rotary_tables(positions: torch.Tensor, inv_freq: torch.Tensor, dtype: torch.
             return rotary_tables(positions, inv_freq, dtype, factor, interleaved)
     positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
     half = inv_freq.shape[0]
-    both = torch.empty((2,) + positions.shape + (2 * half,), dtype=dtype, device=dev)
-    cos, sin = both[0], both[1]
+    both = inv_freq.new_empty((2,) + positions.shape + (2 * half,), dtype=dtype)
+    cos, sin = both.select(0, 0), both.select(0, 1)
     rc = _lib.load().ff_rotary_tables(positions.data_ptr(), positions.numel(), inv_freq.data_ptr(), half, float(factor),
                                       1 if interleaved else 0, code, cos.data_ptr(), sin.data_ptr(), _lib.stream_ptr()) if half and positions.numel() else 0
     if rc:
@@ -97,28 +100,35 @@ def rotary_tables(positions: torch.Tensor, inv_freq: torch.Tensor, dtype: torch.
 
 
 def _apply(query, key, cos, sin, sections, interleaved, transpose):
-    dev = query.device
-    if dev.index != _get_device():
+    dev = query.get_device()
+    if dev != _get_device():
         with torch.cuda.device(dev):
             return _apply(query, key, cos, sin, sections, interleaved, transpose)
-    if query.stride(-1) != 1:
+    qb, qh, qn, last = query.stride()
+    if last != 1:
         query = query.contiguous()
-    if key.stride(-1) != 1:
+        qb, qh, qn, _ = query.stride()
+    kb, kh, kn, last = key.stride()
+    if last != 1:
         key = key.contiguous()
+        kb, kh, kn, _ = key.stride()
     B, H, L, dh = query.shape
-    tshape, tst = cos.shape, cos.stride()
-    q_out, k_out = torch.empty_like(query), torch.empty_like(key)
-    if q_out.stride(-1) != 1:                       # (a dense input whose channels come first in memory order of a size-1 kind)
+    q_out, k_out = torch.empty_like(query), torch.empty_like(key)          # (in the inputs' own order where they are dense)
+    qob, qoh, qon, last = q_out.stride()
+    if last != 1:
         q_out = torch.empty_like(query, memory_format=torch.contiguous_format)
-    if k_out.stride(-1) != 1:
+        qob, qoh, qon, _ = q_out.stride()
+    kob, koh, kon, last = k_out.stride()
+    if last != 1:
         k_out = torch.empty_like(key, memory_format=torch.contiguous_format)
-    qs, ks, qo, ko = query.stride(), key.stride(), q_out.stride(), k_out.stride()
+        kob, koh, kon, _ = k_out.stride()
+    shape, st = cos.shape, cos.stride()
     args = _lib.ROTARY.pack(query.data_ptr(), key.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), cos.data_ptr(), sin.data_ptr(),
-                            _lib.DTYPE_CODE[query.dtype], _lib.DTYPE_CODE[cos.dtype], B, L, H, key.shape[1], dh, tshape[-1],
-                            qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], qo[0], qo[1], qo[2], ko[0], ko[1], ko[2],
-                            tst[0] if len(tshape) == 4 else 0, tst[-3] if tshape[-3] > 1 else 0, tst[-2],
+                            _CODE[query.dtype], _CODE[cos.dtype], B, L, H, key.shape[1], dh, shape[-1],
+                            qb, qh, qn, kb, kh, kn, qob, qoh, qon, kob, koh, kon,
+                            st[0] if len(shape) == 4 else 0, st[-3] if shape[-3] > 1 else 0, st[-2],
                             sections[0] if sections else 0, sections[1] if sections else 0, 1 if interleaved else 0, 1 if transpose else 0,
-                            _lib.stream_ptr())
+                            _raw_stream(dev))
     if B and L:
         rc = _lib.load().ff_rotary_apply(args)
         if rc:
@@ -139,7 +149,8 @@ class _Rotary(torch.autograd.Function):
     def backward(ctx, dq, dk):
         cos, sin = ctx.saved_tensors
         sections, interleaved, transpose = ctx.how
-        dq, dk = _Rotary.apply(dq, dk, cos, sin, sections, interleaved, not transpose)
+        turn = _Rotary.apply if torch.is_grad_enabled() else _apply           # (differentiated again, or the end of the line)
+        dq, dk = turn(dq, dk, cos, sin, sections, interleaved, not transpose)
         return dq, dk, None, None, None, None, None
 
 
@@ -152,18 +163,17 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor, cos: torch.Tensor, sin:
 
     Differentiable in query and key (the tables are constants).  A differentiable call is not captured into a graph: capture
     ``transpose=True`` calls on the gradients instead."""
-    qs, ks, cs = query.shape, key.shape, cos.shape
+    qs, ks, cs, dtype, dev = query.shape, key.shape, cos.shape, query.dtype, query.get_device()
     if len(qs) != 4 or len(ks) != 4 or qs[0] != ks[0] or qs[2:] != ks[2:]:
         raise FrameFusionHipError(f"apply_rotary: query {tuple(qs)} and key {tuple(ks)} must be [B, H, L, dh] and [B, H_kv, L, dh]")
-    if query.dtype not in _lib.DTYPE_CODE or key.dtype != query.dtype:
-        raise FrameFusionHipError(f"apply_rotary: dtypes {query.dtype} / {key.dtype} must be the same of float32, bfloat16, float16")
-    if cos.dtype not in (query.dtype, torch.float32) or sin.dtype != cos.dtype or sin.shape != cs:
+    if dtype not in _CODE or key.dtype is not dtype:
+        raise FrameFusionHipError(f"apply_rotary: dtypes {dtype} / {key.dtype} must be the same of float32, bfloat16, float16")
+    if cos.dtype is not dtype and cos.dtype is not torch.float32 or sin.dtype is not cos.dtype or sin.shape != cs:
         raise FrameFusionHipError("apply_rotary: cos and sin must have one shape and the inputs' dtype or float32")
-    dev = query.device
-    if key.device != dev or cos.device != dev or sin.device != dev:
+    if key.get_device() != dev or cos.get_device() != dev or sin.get_device() != dev:
         raise FrameFusionHipError("apply_rotary: all tensors must be on one device")
     if sections is not None:
-        sections = tuple(int(x) for x in sections)
+        sections = tuple([int(x) for x in sections])
         if len(sections) != 3 or min(sections) < 1 or len(cs) != 4 or cs[0] != 3 or 2 * sum(sections) != cs[-1] or interleaved:
             raise FrameFusionHipError(f"apply_rotary: sections {sections} need tables [3, B, L, 2 * sum] in the half layout, got {tuple(cs)}")
     elif len(cs) != 3:
@@ -172,11 +182,11 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor, cos: torch.Tensor, sin:
         raise FrameFusionHipError(f"apply_rotary: tables {tuple(cs)} do not fit query {tuple(qs)}")
     if cos.requires_grad or sin.requires_grad:
         raise FrameFusionHipError("apply_rotary: the tables are constants, they have no gradient")
-    if dev.type != "cuda":
+    if dev < 0:
         _lib.require_gpu(query, "apply_rotary")
     if cos.stride(-1) != 1 or sin.stride() != cos.stride():
         cos, sin = cos.contiguous(), sin.contiguous()
-    if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad):
+    if (query.requires_grad or key.requires_grad) and torch.is_grad_enabled():
         if torch.cuda.is_current_stream_capturing():
             raise FrameFusionHipError("apply_rotary: a differentiable call cannot be captured into a graph (use transpose=True on the gradients)")
         return _Rotary.apply(query, key, cos, sin, sections, interleaved, transpose)
