@@ -506,17 +506,18 @@ __global__ __launch_bounds__(64 * kAttWaves, DH * NT * (STORE == kStoreSame ? Ac
     }
 }
 
-// Joins the splits of query rows, 32 lanes (dh / 4) to a row and kGroup such groups to share its splits: many for the few rows and many
-// splits of single tokens, one where there are rows enough.  The sums meet in fixed order.
+// Joins the splits of query rows: kLanes lanes take 4 channels each of a row (or a piece of it), kGroup such groups share its splits.
+// Rows enough: a group for the whole row.  The few rows and many splits of single tokens: 32 channels a workgroup and 32 groups over
+// the splits, so that 28 rows of 256 splits are 112 workgroups of 8 loads a thread.  The sums meet in fixed order.
 constexpr int kJoinThreads = 256;
-template <int DT, int DH, int kGroup>
+template <int DT, int DH, int kLanes, int kGroup>
 __global__ __launch_bounds__(kJoinThreads) void k_cache_attention_join(const ff_cache_attention_t a, const AttPlan p) {
-    constexpr int kUnits = DH / 4, kRows = kJoinThreads / kUnits / kGroup;
-    __shared__ f32x4 s_o[kRows * kGroup][kUnits];
+    constexpr int kPieces = DH / 4 / kLanes, kRows = kJoinThreads / kLanes / kGroup;
+    __shared__ f32x4 s_o[kRows * kGroup][kLanes];
     __shared__ float s_l[kRows * kGroup], s_m[kRows * kGroup];
     const ff_cache_t& c = a.cache;
-    const int u = threadIdx.x % kUnits, g = threadIdx.x / kUnits, y = g % kGroup, head = blockIdx.y, b = blockIdx.z;
-    const int r = blockIdx.x * kRows + g / kGroup;
+    const int lane = threadIdx.x % kLanes, g = threadIdx.x / kLanes, y = g % kGroup, head = blockIdx.y, b = blockIdx.z;
+    const int u = blockIdx.x % kPieces * kLanes + lane, r = blockIdx.x / kPieces * kRows + g / kGroup;
     Share share = {b, 0, 1, 0};
     if (c.B == 1) share.used = max(1, min(p.want, blocks_of(c, p, 0)));
     else share_of(c, p, 0, b, share);
@@ -537,8 +538,8 @@ __global__ __launch_bounds__(kJoinThreads) void k_cache_attention_join(const ff_
         sum += x.y * w;
     }
     if constexpr (kGroup > 1) {
-        s_o[g][u] = acc;
-        if (u == 0) s_l[g] = sum, s_m[g] = top;
+        s_o[g][lane] = acc;
+        if (lane == 0) s_l[g] = sum, s_m[g] = top;
         __syncthreads();
         if (y) return;
         float most = kNone;
@@ -550,7 +551,7 @@ __global__ __launch_bounds__(kJoinThreads) void k_cache_attention_join(const ff_
 #pragma unroll
         for (int k = 0; k < kGroup; ++k) {
             const float w = __builtin_amdgcn_exp2f(s_m[g + k] - base);
-            acc += s_o[g + k][u] * w;
+            acc += s_o[g + k][lane] * w;
             sum += s_l[g + k] * w;
         }
     }
@@ -636,17 +637,18 @@ static int launch_attention_dh(const ff_cache_attention_t* a, const AttPlan& p) 
         default: return launch_attention<DT, STORE, 256>(a, p);
     }
 }
-template <int DT, int DH, int kGroup>
+template <int DT, int DH, int kLanes, int kGroup>
 static int launch_join_groups(const ff_cache_attention_t* a, const AttPlan& p) {
-    constexpr int kRows = kJoinThreads / (DH / 4) / kGroup;
-    const dim3 grid((uint32_t)((p.R + kRows - 1) / kRows), (uint32_t)a->cache.kv_heads, (uint32_t)a->cache.B);
-    k_cache_attention_join<DT, DH, kGroup><<<grid, kJoinThreads, 0, (hipStream_t)a->stream>>>(*a, p);
+    constexpr int kRows = kJoinThreads / kLanes / kGroup;
+    const dim3 grid((uint32_t)((p.R + kRows - 1) / kRows * (DH / 4 / kLanes)), (uint32_t)a->cache.kv_heads, (uint32_t)a->cache.B);
+    k_cache_attention_join<DT, DH, kLanes, kGroup><<<grid, kJoinThreads, 0, (hipStream_t)a->stream>>>(*a, p);
     return (int)hipGetLastError();
 }
 template <int DT, int DH>
 static int launch_join(const ff_cache_attention_t* a, const AttPlan& p) {
-    constexpr int kMost = kJoinThreads / (DH / 4);          // a workgroup a row
-    return a->cache.B * a->cache.kv_heads * p.R >= 1024 ? launch_join_groups<DT, DH, 1>(a, p) : launch_join_groups<DT, DH, kMost>(a, p);
+    if (a->cache.B * a->cache.kv_heads * p.R >= 1024) return launch_join_groups<DT, DH, DH / 4, 1>(a, p);
+    // (28 rows: 256 slots 8.4 us with the rows whole, 3.5 us in pieces; 33 slots 3.2 and 4.0)
+    return p.slots > 64 ? launch_join_groups<DT, DH, 8, 32>(a, p) : launch_join_groups<DT, DH, DH / 4, kJoinThreads / (DH / 4)>(a, p);
 }
 template <int DT>
 static int launch_attention_t(const ff_cache_attention_t* a, const AttPlan& p) {
