@@ -49,70 +49,73 @@ __device__ inline uint32_t block_prepare(float* x) {
     return (uint32_t)(e + 127);
 }
 
-// One token to a workgroup: unit threadIdx.x (8 channels) of rows threadIdx.y, + blockDim.y, ...; a row is a key or value of one
-// kv head.  The token's page is looked up once for all its rows.
-template <int DT, int STORE>
-__global__ __launch_bounds__(kRowThreads) void k_cache_write(const ff_cache_rows_t a) {
+// Unit threadIdx.x (8 channels) of a row, a key or value of one kv head of one token.
+// kChunk = 0, few tokens: a token to a workgroup, its rows threadIdx.y, + blockDim.y, ..; the page is looked up once for all of them.
+// kChunk > 0: kChunk times blockDim.y consecutive tokens of ONE row (blockIdx.y) to a workgroup, kChunk in flight a thread: then what a
+// workgroup writes is whole lines, also of the scales (4 bytes a token at 128 channels), which otherwise go out in pieces from the
+// L2s of different XCDs.
+template <int DT, int STORE, int kChunk, bool kWrite>
+__global__ __launch_bounds__(kRowThreads) void k_cache_rows(const ff_cache_rows_t a) {
+    constexpr int kTokens = kChunk ? kChunk : 1;
     const ff_cache_t& c = a.cache;
-    const uint32_t tok = blockIdx.x, b = tok / (uint32_t)c.n, t = tok - b * (uint32_t)c.n;
+    const uint32_t n = (uint32_t)c.n, step = kChunk ? blockDim.y : 1, per = (n + kTokens * step - 1) / (kTokens * step);
+    const uint32_t b = blockIdx.x / per, t0 = (blockIdx.x - b * per) * kTokens * step + (kChunk ? threadIdx.y : 0);
     const int start = c.start[b];
-    if (start < 0) return;
+    if (kWrite && start < 0) return;
     const int kv = (int)c.kv_heads, dh = (int)c.dh, u = threadIdx.x;
-    const int64_t row0 = cache_row(c.table + (int64_t)b * c.table_width, c.table_width, c.n_pages, (int)c.page_size, kv, 0, (int64_t)start + t);
-    if (row0 < 0) return;
-    for (int r = threadIdx.y; r < 2 * kv; r += blockDim.y) {
+    int64_t row0[kTokens];
+#pragma unroll
+    for (int k = 0; k < kTokens; ++k)
+        row0[k] = start < 0 || t0 + k * step >= n ? -1 : cache_row(c.table + (int64_t)b * c.table_width, c.table_width, c.n_pages, (int)c.page_size, kv, 0,
+                                                                  (int64_t)start + t0 + k * step);
+    for (int r = kChunk ? blockIdx.y : threadIdx.y; r < 2 * kv; r += kChunk ? 2 * kv : blockDim.y) {
         const bool is_v = r >= kv;
         const int h = is_v ? r - kv : r;
-        const char* src = (const char*)(is_v ? a.v : a.k) +
-            ((is_v ? (int64_t)b * a.v_batch + h * a.v_head + t * a.v_token : (int64_t)b * a.k_batch + h * a.k_head + t * a.k_token) + u * 8) * Act<DT>::kBytes;
-        const int64_t row = row0 + (int64_t)h * c.page_size;
-        char* dst = (char*)(is_v ? c.values : c.keys) + row * row_bytes<DT, STORE>(dh);
-        if constexpr (STORE == kStoreSame) {
-            const uint4* s = (const uint4*)src;
-            uint4* d = (uint4*)(dst + u * 8 * Act<DT>::kBytes);
-            d[0] = s[0];
-            if constexpr (DT == FF_F32) d[1] = s[1];
-        } else {
-            float x[8];
-            load8<DT>(src, x);
-            const uint32_t byte = block_prepare<DT, STORE>(x);
-            if constexpr (STORE == FF_STORE_E4M3) {
-                int lo = 0, hi = 0;
-                lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], lo, false);
-                lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], lo, true);
-                hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[4], x[5], hi, false);
-                hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[6], x[7], hi, true);
-                ((uint2*)dst)[u] = make_uint2((uint32_t)lo, (uint32_t)hi);
-            } else {
-                uint32_t w = 0;
-                w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], 1.0f, 0);
-                w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], 1.0f, 1);
-                w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], 1.0f, 2);
-                w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], 1.0f, 3);
-                ((uint32_t*)dst)[u] = w;
-            }
-            if ((u & 3) == 0) (is_v ? c.value_scales : c.key_scales)[row * (dh / 32) + u / 4] = (uint8_t)byte;
+        const int64_t token = (is_v ? a.v_token : a.k_token) * step;
+        char* mine = (char*)(is_v ? a.v : a.k) +
+            ((is_v ? (int64_t)b * a.v_batch + h * a.v_head : (int64_t)b * a.k_batch + h * a.k_head) + t0 * (is_v ? a.v_token : a.k_token) + u * 8) * Act<DT>::kBytes;
+        void* codes = is_v ? c.values : c.keys;
+        uint8_t* scales = is_v ? c.value_scales : c.key_scales;
+        float x[kTokens][8];
+#pragma unroll
+        for (int k = 0; k < kTokens; ++k) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[k][e] = 0.f;
+            if (row0[k] < 0) continue;
+            if constexpr (kWrite) load8<DT>(mine + k * token * Act<DT>::kBytes, x[k]);
+            else fetch8<DT, STORE>(codes, scales, row0[k] + (int64_t)h * c.page_size, dh, u, x[k]);
         }
-    }
-}
-
-template <int DT, int STORE>
-__global__ __launch_bounds__(kRowThreads) void k_cache_read(const ff_cache_rows_t a) {
-    const ff_cache_t& c = a.cache;
-    const uint32_t tok = blockIdx.x, b = tok / (uint32_t)c.n, t = tok - b * (uint32_t)c.n;
-    const int start = c.start[b];
-    const int kv = (int)c.kv_heads, dh = (int)c.dh, u = threadIdx.x;
-    const int64_t row0 = start < 0 ? -1 : cache_row(c.table + (int64_t)b * c.table_width, c.table_width, c.n_pages, (int)c.page_size, kv, 0,
-                                                    (int64_t)start + t);
-    for (int r = threadIdx.y; r < 2 * kv; r += blockDim.y) {
-        const bool is_v = r >= kv;
-        const int h = is_v ? r - kv : r;
-        char* dst = (char*)(is_v ? a.v : a.k) +
-            ((is_v ? (int64_t)b * a.v_batch + h * a.v_head + t * a.v_token : (int64_t)b * a.k_batch + h * a.k_head + t * a.k_token) + u * 8) * Act<DT>::kBytes;
-        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (row0 >= 0)
-            fetch8<DT, STORE>(is_v ? c.values : c.keys, is_v ? c.value_scales : c.key_scales, row0 + (int64_t)h * c.page_size, dh, u, x);
-        store8<DT>(dst, x);
+#pragma unroll
+        for (int k = 0; k < kTokens; ++k) {
+            if constexpr (!kWrite) {
+                if (t0 + k * step < n) store8<DT>(mine + k * token * Act<DT>::kBytes, x[k]);
+                continue;
+            }
+            if (row0[k] < 0) continue;                       // (the same for all lanes of a block of 32 channels)
+            const int64_t row = row0[k] + (int64_t)h * c.page_size;
+            char* dst = (char*)codes + row * row_bytes<DT, STORE>(dh);
+            if constexpr (STORE == kStoreSame) {
+                store8<DT>(dst + u * 8 * Act<DT>::kBytes, x[k]);
+            } else {
+                const uint32_t byte = block_prepare<DT, STORE>(x[k]);
+                if constexpr (STORE == FF_STORE_E4M3) {
+                    int lo = 0, hi = 0;
+                    lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[k][0], x[k][1], lo, false);
+                    lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[k][2], x[k][3], lo, true);
+                    hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[k][4], x[k][5], hi, false);
+                    hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[k][6], x[k][7], hi, true);
+                    ((uint2*)dst)[u] = make_uint2((uint32_t)lo, (uint32_t)hi);
+                } else {
+                    uint32_t w = 0;
+                    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[k][0], x[k][1], 1.0f, 0);
+                    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[k][2], x[k][3], 1.0f, 1);
+                    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[k][4], x[k][5], 1.0f, 2);
+                    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[k][6], x[k][7], 1.0f, 3);
+                    ((uint32_t*)dst)[u] = w;
+                }
+                if ((u & 3) == 0) scales[row * (dh / 32) + u / 4] = (uint8_t)byte;
+            }
+        }
     }
 }
 
@@ -178,11 +181,18 @@ static int rows_check(const ff_cache_rows_t* a) {
 template <int DT, int STORE>
 static int launch_rows(const ff_cache_rows_t* a, bool write) {
     const ff_cache_t& c = a->cache;
-    const int units = (int)c.dh / 8;
-    const int y = min(kRowThreads / units, (int)(2 * c.kv_heads));
-    const dim3 block(units, y), grid((uint32_t)(c.B * c.n));
-    if (write) k_cache_write<DT, STORE><<<grid, block, 0, (hipStream_t)a->stream>>>(*a);
-    else k_cache_read<DT, STORE><<<grid, block, 0, (hipStream_t)a->stream>>>(*a);
+    const int units = (int)c.dh / 8, most = kRowThreads / units;
+    hipStream_t st = (hipStream_t)a->stream;
+    if (c.n >= most) {
+        constexpr int kChunk = 2;
+        const dim3 block(units, most), grid((uint32_t)(c.B * ((c.n + kChunk * most - 1) / (kChunk * most))), (uint32_t)(2 * c.kv_heads));
+        if (write) k_cache_rows<DT, STORE, kChunk, true><<<grid, block, 0, st>>>(*a);
+        else k_cache_rows<DT, STORE, kChunk, false><<<grid, block, 0, st>>>(*a);
+    } else {
+        const dim3 block(units, min(most, (int)(2 * c.kv_heads))), grid((uint32_t)(c.B * c.n));
+        if (write) k_cache_rows<DT, STORE, 0, true><<<grid, block, 0, st>>>(*a);
+        else k_cache_rows<DT, STORE, 0, false><<<grid, block, 0, st>>>(*a);
+    }
     return (int)hipGetLastError();
 }
 template <int DT>
