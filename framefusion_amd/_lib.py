@@ -16,6 +16,7 @@ import torch  # noqa: F401  (must precede the CDLL below)
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libframefusion_hip.so")
+HOST_PATH = os.path.join(_HERE, "_host.so")
 CSRC = os.path.join(_HERE, "csrc")
 
 FF_F32, FF_BF16, FF_F16 = 0, 1, 2
@@ -312,6 +313,24 @@ def load():
                                       f"{lib.ff_abi_sizeof(which)} in the library")
     _lib = lib
     return lib
+
+
+_host = None
+
+
+def host():
+    """framefusion_amd._host (csrc/ff_host.cpp, built with the library): the cached-decoding calls in one crossing each."""
+    global _host
+    if _host is None:
+        load()                               # (rebuilds both when the sources have changed)
+        if not os.path.exists(HOST_PATH):
+            build()
+        try:
+            import importlib
+            _host = importlib.import_module("framefusion_amd._host")
+        except ImportError as e:
+            raise FrameFusionHipError(f"cannot load {HOST_PATH}: {e} (built with another torch? run `make -C {CSRC}`); there is no other path") from e
+    return _host
 
 
 def check(rc: int, what: str):

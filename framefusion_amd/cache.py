@@ -22,10 +22,7 @@ import torch
 from . import _lib
 from ._lib import FrameFusionHipError
 
-_get_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 _STORES = {"fp8": torch.float8_e4m3fn, "fp4": torch.uint8}
-_STORE_CODE = {torch.float8_e4m3fn: _lib.STORE_E4M3, torch.uint8: _lib.STORE_E2M1, torch.float32: _lib.FF_F32,
-               torch.bfloat16: _lib.FF_BF16, torch.float16: _lib.FF_F16}
 
 
 class CacheTensors(NamedTuple):
@@ -52,125 +49,23 @@ def new_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: t
     return CacheTensors(keys, values, *(torch.zeros(rows + (head_dim // 32,), dtype=torch.uint8, device=device) for _ in range(2)))
 
 
-_CODE = _lib.DTYPE_CODE
-_UINT8, _INT32 = torch.uint8, torch.int32
-
-
-def _head(what, cache, table, start, n, dtype):
-    """The fields of ff_cache_t, every one checked, and the device's index."""
-    keys, values, key_scales, value_scales = cache
-    shape, store, code, dev = keys.shape, _STORE_CODE.get(keys.dtype), _CODE.get(dtype), keys.get_device()
-    if (store is None or code is None or len(shape) != 4 or values.shape != shape or values.dtype is not keys.dtype or values.get_device() != dev
-            or not keys.is_contiguous() or not values.is_contiguous()):
-        raise FrameFusionHipError(f"{what}: keys and values of a cache must be alike and contiguous, [pages, kv_heads, page_size, head_dim], and serve "
-                                  f"float32, bfloat16 or float16, not {dtype}")
-    pages, kv_heads, page_size, head_dim = shape
-    if store == code:
-        if key_scales is not None or value_scales is not None:
-            raise FrameFusionHipError(f"{what}: a cache in {dtype} holds no scales")
-        ks = vs = 0
-    else:
-        if store < 4:
-            raise FrameFusionHipError(f"{what}: a cache in {keys.dtype} serves that type alone, not {dtype}")
-        if store == 4:
-            head_dim *= 2
-        want = (pages, kv_heads, page_size, head_dim // 32)
-        if (key_scales is None or value_scales is None or key_scales.shape != want or value_scales.shape != want or key_scales.dtype is not _UINT8
-                or value_scales.dtype is not _UINT8 or not key_scales.is_contiguous() or not value_scales.is_contiguous()
-                or key_scales.get_device() != dev or value_scales.get_device() != dev):
-            raise FrameFusionHipError(f"{what}: a cache of codes needs contiguous uint8 scales {want}")
-        ks, vs = key_scales.data_ptr(), value_scales.data_ptr()
-    ts = table.shape
-    if (len(ts) != 2 or table.dtype is not _INT32 or start.dtype is not _INT32 or start.shape != ts[:1] or table.get_device() != dev
-            or start.get_device() != dev or not table.is_contiguous() or not start.is_contiguous()):
-        raise FrameFusionHipError(f"{what}: table must be int32 [B, width] and start int32 [B], contiguous, on the cache's device")
-    if dev < 0:
-        _lib.require_gpu(keys, what)
-    return (keys.data_ptr(), values.data_ptr(), ks, vs, table.data_ptr(), start.data_ptr(), store, pages, kv_heads, page_size, head_dim,
-            ts[1], ts[0], n, code), dev
-
-
-def _no_gradient(what, *tensors):
-    if any([t.requires_grad for t in tensors]) and torch.is_grad_enabled():
-        raise FrameFusionHipError(f"{what} has no gradient (serving only): call it under torch.no_grad()")
-
-
-def _rows(t):
-    """`t` [B, heads, n, dh] itself if the kernels can read it in place, else a contiguous copy; strides of batch, head and token
-    (that of a dimension of one is never used)."""
-    b, h, n, last = t.stride()
-    sb, sh, sn, _ = t.shape
-    if sb == 1:
-        b = 0
-    if sh == 1:
-        h = 0
-    if sn == 1:
-        n = 0
-    if last != 1 or (b | h | n) % (16 // t.element_size()) or t.data_ptr() & 15:
-        t = t.clone(memory_format=torch.contiguous_format)
-        b, h, n, _ = t.stride()
-    return t, b, h, n
-
-
 def cache_write(cache, key: torch.Tensor, value: torch.Tensor, table: torch.Tensor, start: torch.Tensor) -> None:
     """Stores key and value [B, kv_heads, n, head_dim] at positions start[b] .. start[b] + n - 1 of each sequence (rounded to the
     cache's 8 or 4 bits on the way).  Positions without a page and padding rows are left out; nothing else changes."""
-    _no_gradient("cache_write", key, value)
-    head, dev = _head("cache_write", cache, table, start, key.shape[2] if key.ndim == 4 else -1, key.dtype)
-    want = (head[12], head[8], head[13], head[10])
-    if key.shape != want or value.shape != want or value.dtype is not key.dtype or key.get_device() != dev or value.get_device() != dev:
-        raise FrameFusionHipError(f"cache_write: key and value must be {want} of one dtype on the cache's device, got {tuple(key.shape)} and {tuple(value.shape)}")
-    if dev != _get_device():
-        with torch.cuda.device(dev):
-            return cache_write(cache, key, value, table, start)
-    if 0 in want:
-        return
-    key, kb, kh, kt = _rows(key)
-    value, vb, vh, vt = _rows(value)
-    rc = _lib.load().ff_cache_write(_lib.CACHE_ROWS.pack(*head, key.data_ptr(), value.data_ptr(), kb, kh, kt, vb, vh, vt, _raw_stream(dev)))
-    if rc:
-        _lib.check(rc, "ff_cache_write")
+    _lib.host().write(cache, key, value, table, start)
 
 
 def cache_read(cache, table: torch.Tensor, start: torch.Tensor, count: int, dtype: Optional[torch.dtype] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """(key, value) [B, kv_heads, count, head_dim] of ``dtype`` (the cache's own, or bfloat16 for one of codes): the values of
     positions start[b] .. start[b] + count - 1; zeros where a position has no page and in padding rows."""
-    if count < 0:
-        raise FrameFusionHipError("cache_read: count must not be negative")
-    if dtype is None:
-        dtype = cache[0].dtype if cache[0].dtype in _lib.DTYPE_CODE else torch.bfloat16
-    head, dev = _head("cache_read", cache, table, start, count, dtype)
-    if dev != _get_device():
-        with torch.cuda.device(dev):
-            return cache_read(cache, table, start, count, dtype)
-    B, kv_heads, dh = head[12], head[8], head[10]
-    both = cache[0].new_empty((2, B, kv_heads, count, dh), dtype=dtype)
-    key, value = both.select(0, 0), both.select(0, 1)
-    if B and kv_heads and count:
-        t = count * dh
-        rc = _lib.load().ff_cache_read(_lib.CACHE_ROWS.pack(*head, key.data_ptr(), value.data_ptr(), kv_heads * t, t, dh, kv_heads * t, t, dh, _raw_stream(dev)))
-        if rc:
-            _lib.check(rc, "ff_cache_read")
-    return key, value
+    return _lib.host().read(cache, table, start, count, dtype)
 
 
 def cache_keep(cache, table: torch.Tensor, start: torch.Tensor, accepted: torch.Tensor) -> None:
     """Keeps the accepted ones of the tokens written behind start[b]: row start[b] + i becomes a copy of row
     start[b] + accepted[b, i].  ``accepted`` int32 [B, m], each list strictly increasing; it ends at the first entry that is negative
     (or out of order, or without a page).  The caller then holds start[b] + (length of the list) tokens."""
-    dtype = cache[0].dtype
-    head, dev = _head("cache_keep", cache, table, start, 0, dtype if dtype in _CODE else torch.bfloat16)
-    shape = accepted.shape
-    if accepted.dtype is not _INT32 or len(shape) != 2 or shape[0] != head[12] or accepted.get_device() != dev or not accepted.is_contiguous():
-        raise FrameFusionHipError("cache_keep: accepted must be a contiguous int32 [B, m] on the cache's device")
-    if dev != _get_device():
-        with torch.cuda.device(dev):
-            return cache_keep(cache, table, start, accepted)
-    if 0 in shape:
-        return
-    rc = _lib.load().ff_cache_keep(_lib.CACHE.pack(*head), accepted.data_ptr(), shape[1], _raw_stream(dev))
-    if rc:
-        _lib.check(rc, "ff_cache_keep")
+    _lib.host().keep(cache, table, start, accepted)
 
 
 def cache_attention(query: torch.Tensor, cache, table: torch.Tensor, start: torch.Tensor, mask: Optional[torch.Tensor] = None,
@@ -182,37 +77,7 @@ def cache_attention(query: torch.Tensor, cache, table: torch.Tensor, start: torc
 
     H is a multiple of the cache's heads, head_dim 32, 64, 128 or 256.  Returns [B, H, n, head_dim], laid out so that
     ``out.transpose(1, 2)`` is contiguous."""
-    _no_gradient("cache_attention", query)
-    if query.ndim != 4:
-        raise FrameFusionHipError(f"cache_attention: query must be [B, H, n, head_dim], got {tuple(query.shape)}")
-    B, H, n, dh = query.shape
-    if mask is not None and (mask.dtype is not torch.bool or mask.get_device() != query.get_device() or mask.shape not in ((n, n), (B, n, n))):
-        raise FrameFusionHipError(f"cache_attention: mask must be bool [{n}, {n}] or [{B}, {n}, {n}], got {mask.dtype} {tuple(mask.shape)}")
-    if dh not in (32, 64, 128, 256):
-        raise FrameFusionHipError(f"cache_attention: head_dim must be 32, 64, 128 or 256, got {dh}")
-    head, dev = _head("cache_attention", cache, table, start, n, query.dtype)
-    if B != head[12] or dh != head[10] or H < 1 or H % head[8] or dev != query.get_device():
-        raise FrameFusionHipError(f"cache_attention: query {tuple(query.shape)} does not fit a table of {head[12]} sequences and {head[8]} heads of {head[10]}")
-    if dev != _get_device():
-        with torch.cuda.device(dev):
-            return cache_attention(query, cache, table, start, mask, scale)
-    mask_ptr = mask_batch = 0
-    if mask is not None:
-        mask = mask.contiguous()
-        mask_ptr, mask_batch = mask.data_ptr(), n * n if mask.ndim == 3 else 0
-    out = query.new_empty((B, n, H, dh))
-    if B and n:
-        query, qb, qh, qn = _rows(query)
-        lib = _lib.load()
-        scale = dh ** -0.5 if scale is None else float(scale)
-        fields = (*head, query.data_ptr(), out.data_ptr(), mask_ptr)
-        rest = (H, qb, qh, qn, n * H * dh, dh, H * dh, mask_batch, scale, _raw_stream(dev))
-        need = lib.ff_cache_attention_workspace_bytes(_lib.CACHE_ATTENTION.pack(*fields, 0, 0, *rest))
-        ws = query.new_empty((need,), dtype=_UINT8) if need else None
-        rc = lib.ff_cache_attention(_lib.CACHE_ATTENTION.pack(*fields, ws.data_ptr() if need else 0, need, *rest))
-        if rc:
-            _lib.check(rc, "ff_cache_attention")
-    return out.transpose(1, 2)
+    return _lib.host().attention(query, cache, table, start, mask, scale)
 
 
 class ReducedCache:

@@ -57,7 +57,8 @@ struct AttPlan {                    // what the host derives once a call
     uint32_t magic;                 // ... and floor(2^32 / page16) (2^32 - 1 for 1)
     float scale2;                   // |scale| log2(e), at least the smallest normal number (0 times a masked score would be NaN)
     uint32_t flip;                  // scale < 0: sign bits of two elements of 16-bit Q, taken up there (fp32: of one)
-    float* part;                    // slots > 1: [kv heads, R, slots] x DH sums, then as many (maximum, sum) pairs
+    float* part;                    // slots > 1: [kv heads, R, slots] x DH sums, then as many (maximum, sum) pairs, then
+    int2* shares;                   // (first slot, splits) of each sequence, written by its split 0 for the join
     int64_t part_rows;
 };
 
@@ -74,7 +75,7 @@ struct Share { int b, split, used, first; };
 // one sequence, or none split: known at once but for `used`, so a kernel's first loads need not wait for the lengths
 __device__ inline bool plain_share(const ff_cache_t& c, const AttPlan& p) { return c.B == 1 || p.slots == 1; }
 __device__ inline int blocks_of(const ff_cache_t& c, const AttPlan& p, int b) { return (int)((keys_of(c, c.start[b]) + p.block - 1) / p.block); }
-__device__ inline bool share_of(const ff_cache_t& c, const AttPlan& p, int w, int of_b, Share& s) {
+__device__ inline bool share_of(const ff_cache_t& c, const AttPlan& p, int w, Share& s) {
     const int B = (int)c.B, lane = threadIdx.x & 63;
     auto sum = [&](int each) {                    // blocks of all sequences, or with each > 0 their splits of so many
         int64_t x = 0;
@@ -95,13 +96,13 @@ __device__ inline bool share_of(const ff_cache_t& c, const AttPlan& p, int w, in
     for (int b0 = 0; b0 < B; b0 += 64) {
         const int b = b0 + lane, used = b < B ? max(1, (blocks_of(c, p, b) + each - 1) / each) : 0;
         const int incl = wave_incl_scan_dpp(used);
-        const uint64_t found = of_b < 0 ? __ballot(b < B && before + incl > w) : __ballot(b == of_b);
+        const uint64_t found = __ballot(b < B && before + incl > w);
         if (found) {
             const int l = __ffsll((long long)found) - 1;
             s.b = b0 + l;
             s.used = __builtin_amdgcn_readlane(used, l);
             s.first = before + __builtin_amdgcn_readlane(incl, l) - s.used;
-            s.split = of_b < 0 ? w - s.first : 0;
+            s.split = w - s.first;
             return true;
         }
         before += __builtin_amdgcn_readlane(incl, 63);

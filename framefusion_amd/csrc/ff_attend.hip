@@ -223,7 +223,7 @@ __global__ __launch_bounds__(64 * kAttWaves, DH * NT * (STORE == kStoreSame ? Ac
     const int head = blockIdx.y / p.groups, group = blockIdx.y - head * p.groups;
     const bool plain = plain_share(c, p);
     Share share = {p.slots == 1 ? (int)blockIdx.x : 0, p.slots == 1 ? 0 : (int)blockIdx.x, 1, 0};
-    if (!plain && !share_of(c, p, blockIdx.x, -1, share)) return;
+    if (!plain && !share_of(c, p, blockIdx.x, share)) return;
     const int b = share.b, split = share.split;
     const int32_t* table = c.table + (int64_t)b * c.table_width;
     int page0, page1, off0, off1;
@@ -461,6 +461,9 @@ __global__ __launch_bounds__(64 * kAttWaves, DH * NT * (STORE == kStoreSame ? Ac
         }
     }
 
+    // (stores stand behind the loop: in front of it the page table could no longer be read as a constant, by scalar loads - 358 us
+    // became 490)
+    if (p.slots > 1 && split == 0 && blockIdx.y == 0 && threadIdx.x == 0) p.shares[b] = make_int2(share.first, share.used);
     // the four waves' rows, joined: channel (4 q + r) kVE + x of row `col` is o[x][r]
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -515,14 +518,11 @@ __global__ __launch_bounds__(kJoinThreads) void k_cache_attention_join(const ff_
     constexpr int kPieces = DH / 4 / kLanes, kRows = kJoinThreads / kLanes / kGroup;
     __shared__ f32x4 s_o[kRows * kGroup][kLanes];
     __shared__ float s_l[kRows * kGroup], s_m[kRows * kGroup];
-    const ff_cache_t& c = a.cache;
     const int lane = threadIdx.x % kLanes, g = threadIdx.x / kLanes, y = g % kGroup, head = blockIdx.y, b = blockIdx.z;
     const int u = blockIdx.x % kPieces * kLanes + lane, r = blockIdx.x / kPieces * kRows + g / kGroup;
-    Share share = {b, 0, 1, 0};
-    if (c.B == 1) share.used = max(1, min(p.want, blocks_of(c, p, 0)));
-    else share_of(c, p, 0, b, share);
-    const int used = r < p.R ? share.used : 0;
-    const int64_t at = ((int64_t)head * p.R + (r < p.R ? r : 0)) * p.slots + share.first;
+    const int2 share = p.shares[b];
+    const int used = r < p.R ? share.y : 0;
+    const int64_t at = ((int64_t)head * p.R + (r < p.R ? r : 0)) * p.slots + share.x;
     const float2* ml = (const float2*)(p.part + p.part_rows * DH) + at;
     const float* part = p.part + at * DH + u * 4;
     float top = kNone;
@@ -615,6 +615,7 @@ static AttPlan attention_plan(const ff_cache_attention_t* a) {
     p.slots = whole ? 1 : (int)(p.want + (c.B > 1 ? c.B : 0));
     p.part_rows = p.slots > 1 ? c.kv_heads * p.R * p.slots : 0;
     p.part = (float*)a->ws;
+    p.shares = p.part ? (int2*)(p.part + p.part_rows * (c.dh + 2)) : nullptr;
     return p;
 }
 
@@ -646,7 +647,8 @@ static int launch_join_groups(const ff_cache_attention_t* a, const AttPlan& p) {
 }
 template <int DT, int DH>
 static int launch_join(const ff_cache_attention_t* a, const AttPlan& p) {
-    if (a->cache.B * a->cache.kv_heads * p.R >= 1024) return launch_join_groups<DT, DH, DH / 4, 1>(a, p);
+    // (6 832 rows of 30 slots: 11 us a group a row, 8 us four)
+    if (a->cache.B * a->cache.kv_heads * p.R >= 1024) return launch_join_groups<DT, DH, DH / 4, DH == 256 ? 2 : 4>(a, p);
     // (28 rows: 256 slots 8.4 us with the rows whole, 3.5 us in pieces; 33 slots 3.2 and 4.0)
     return p.slots > 64 ? launch_join_groups<DT, DH, 8, 32>(a, p) : launch_join_groups<DT, DH, DH / 4, kJoinThreads / (DH / 4)>(a, p);
 }
@@ -674,7 +676,7 @@ static int launch_attention_t(const ff_cache_attention_t* a, const AttPlan& p) {
 extern "C" size_t ff_cache_attention_workspace_bytes(const ff_cache_attention_t* a) {
     if (ff::attention_check(a) || a->cache.B == 0 || a->cache.n == 0) return 0;
     const ff::AttPlan p = ff::attention_plan(a);
-    return (size_t)p.part_rows * (size_t)(a->cache.dh + 2) * sizeof(float);
+    return p.slots > 1 ? (size_t)p.part_rows * (size_t)(a->cache.dh + 2) * sizeof(float) + (size_t)a->cache.B * sizeof(int2) : 0;
 }
 
 extern "C" int ff_cache_attention(const ff_cache_attention_t* a) {

@@ -13,7 +13,7 @@ import torch
 from . import _lib
 from ._lib import FrameFusionHipError
 
-_get_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+_get_device = torch._C._cuda_getDevice
 
 
 _CODE = _lib.DTYPE_CODE
@@ -99,43 +99,6 @@ def rotary_tables(positions: torch.Tensor, inv_freq: torch.Tensor, dtype: torch.
     return cos, sin
 
 
-def _apply(query, key, cos, sin, sections, interleaved, transpose):
-    dev = query.get_device()
-    if dev != _get_device():
-        with torch.cuda.device(dev):
-            return _apply(query, key, cos, sin, sections, interleaved, transpose)
-    qb, qh, qn, last = query.stride()
-    if last != 1:
-        query = query.contiguous()
-        qb, qh, qn, _ = query.stride()
-    kb, kh, kn, last = key.stride()
-    if last != 1:
-        key = key.contiguous()
-        kb, kh, kn, _ = key.stride()
-    B, H, L, dh = query.shape
-    q_out, k_out = torch.empty_like(query), torch.empty_like(key)          # (in the inputs' own order where they are dense)
-    qob, qoh, qon, last = q_out.stride()
-    if last != 1:
-        q_out = torch.empty_like(query, memory_format=torch.contiguous_format)
-        qob, qoh, qon, _ = q_out.stride()
-    kob, koh, kon, last = k_out.stride()
-    if last != 1:
-        k_out = torch.empty_like(key, memory_format=torch.contiguous_format)
-        kob, koh, kon, _ = k_out.stride()
-    shape, st = cos.shape, cos.stride()
-    args = _lib.ROTARY.pack(query.data_ptr(), key.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), cos.data_ptr(), sin.data_ptr(),
-                            _CODE[query.dtype], _CODE[cos.dtype], B, L, H, key.shape[1], dh, shape[-1],
-                            qb, qh, qn, kb, kh, kn, qob, qoh, qon, kob, koh, kon,
-                            st[0] if len(shape) == 4 else 0, st[-3] if shape[-3] > 1 else 0, st[-2],
-                            sections[0] if sections else 0, sections[1] if sections else 0, 1 if interleaved else 0, 1 if transpose else 0,
-                            _raw_stream(dev))
-    if B and L:
-        rc = _lib.load().ff_rotary_apply(args)
-        if rc:
-            _lib.check(rc, "ff_rotary_apply")
-    return q_out, k_out
-
-
 class _Rotary(torch.autograd.Function):
     """y = R x for both inputs; the gradient is R^T (itself a rotation call, so it can be differentiated again)."""
 
@@ -143,13 +106,13 @@ class _Rotary(torch.autograd.Function):
     def forward(ctx, query, key, cos, sin, sections, interleaved, transpose):
         ctx.save_for_backward(cos, sin)
         ctx.how = (sections, interleaved, transpose)
-        return _apply(query, key, cos, sin, sections, interleaved, transpose)
+        return _lib.host().rotary(query, key, cos, sin, sections, interleaved, transpose)
 
     @staticmethod
     def backward(ctx, dq, dk):
         cos, sin = ctx.saved_tensors
         sections, interleaved, transpose = ctx.how
-        turn = _Rotary.apply if torch.is_grad_enabled() else _apply           # (differentiated again, or the end of the line)
+        turn = _Rotary.apply if torch.is_grad_enabled() else _lib.host().rotary           # (differentiated again, or the end of the line)
         dq, dk = turn(dq, dk, cos, sin, sections, interleaved, not transpose)
         return dq, dk, None, None, None, None, None
 
@@ -163,31 +126,8 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor, cos: torch.Tensor, sin:
 
     Differentiable in query and key (the tables are constants).  A differentiable call is not captured into a graph: capture
     ``transpose=True`` calls on the gradients instead."""
-    qs, ks, cs, dtype, dev = query.shape, key.shape, cos.shape, query.dtype, query.get_device()
-    if len(qs) != 4 or len(ks) != 4 or qs[0] != ks[0] or qs[2:] != ks[2:]:
-        raise FrameFusionHipError(f"apply_rotary: query {tuple(qs)} and key {tuple(ks)} must be [B, H, L, dh] and [B, H_kv, L, dh]")
-    if dtype not in _CODE or key.dtype is not dtype:
-        raise FrameFusionHipError(f"apply_rotary: dtypes {dtype} / {key.dtype} must be the same of float32, bfloat16, float16")
-    if cos.dtype is not dtype and cos.dtype is not torch.float32 or sin.dtype is not cos.dtype or sin.shape != cs:
-        raise FrameFusionHipError("apply_rotary: cos and sin must have one shape and the inputs' dtype or float32")
-    if key.get_device() != dev or cos.get_device() != dev or sin.get_device() != dev:
-        raise FrameFusionHipError("apply_rotary: all tensors must be on one device")
-    if sections is not None:
-        sections = tuple([int(x) for x in sections])
-        if len(sections) != 3 or min(sections) < 1 or len(cs) != 4 or cs[0] != 3 or 2 * sum(sections) != cs[-1] or interleaved:
-            raise FrameFusionHipError(f"apply_rotary: sections {sections} need tables [3, B, L, 2 * sum] in the half layout, got {tuple(cs)}")
-    elif len(cs) != 3:
-        raise FrameFusionHipError(f"apply_rotary: tables must be [B or 1, L, rot] (or [3, ...] with sections), got {tuple(cs)}")
-    if cs[-3] not in (1, qs[0]) or cs[-2] != qs[2] or cs[-1] % 2 or not 2 <= cs[-1] <= qs[3]:
-        raise FrameFusionHipError(f"apply_rotary: tables {tuple(cs)} do not fit query {tuple(qs)}")
-    if cos.requires_grad or sin.requires_grad:
-        raise FrameFusionHipError("apply_rotary: the tables are constants, they have no gradient")
-    if dev < 0:
-        _lib.require_gpu(query, "apply_rotary")
-    if cos.stride(-1) != 1 or sin.stride() != cos.stride():
-        cos, sin = cos.contiguous(), sin.contiguous()
     if (query.requires_grad or key.requires_grad) and torch.is_grad_enabled():
-        if torch.cuda.is_current_stream_capturing():
+        if query.is_cuda and torch.cuda.is_current_stream_capturing():
             raise FrameFusionHipError("apply_rotary: a differentiable call cannot be captured into a graph (use transpose=True on the gradients)")
         return _Rotary.apply(query, key, cos, sin, sections, interleaved, transpose)
-    return _apply(query, key, cos, sin, sections, interleaved, transpose)
+    return _lib.host().rotary(query, key, cos, sin, sections, interleaved, transpose)
