@@ -89,7 +89,7 @@ class ReducedCache:
     pending until ``keep(accepted)``.
 
     ``max_tokens`` bounds the length of every layer; ``pages`` the pool (default: enough for ``max_tokens`` everywhere - a reduced
-    prefill needs far fewer).  One instance serves one stream of calls, like the reference's module."""
+    prefill needs far fewer).  One instance serves one stream of calls, like the reference's module; after a step that raised, ``reset``."""
 
     def __init__(self, layers: int, kv_heads: int, head_dim: int, max_tokens: int, dtype: torch.dtype = torch.bfloat16,
                  store: Optional[str] = None, page_size: int = 64, pages: Optional[int] = None, device="cuda"):
@@ -125,6 +125,10 @@ class ReducedCache:
             new = [self._free.pop() for _ in range(more)]
             self._table[layer, len(have):len(have) + more] = torch.tensor(new, dtype=torch.int32)
             have += new
+
+    def update(self, *args, **kwargs):
+        """What a layer that does not know this class would call."""
+        raise FrameFusionHipError("a ReducedCache serves Qwen2 / Qwen2-VL models patched by apply_framefusion; this layer expects a transformers cache")
 
     def append(self, layer: int, key: torch.Tensor, value: torch.Tensor) -> None:
         """Writes key and value [1, kv_heads, n, head_dim] behind the layer's tokens; they count once ``advance`` or ``keep`` is called."""

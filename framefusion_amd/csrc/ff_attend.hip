@@ -565,7 +565,7 @@ static int attention_check(const ff_cache_attention_t* a) {
     if (!a) return FF_ERR_ARG;
     const int rc = cache_check(&a->cache);
     if (rc) return rc;
-    if (!a->q || !a->out || a->H < 1 || a->H % a->cache.kv_heads || a->mask_batch < 0) return FF_ERR_ARG;
+    if ((a->cache.B && a->cache.n && (!a->q || !a->out)) || a->H < 1 || a->H % a->cache.kv_heads || a->mask_batch < 0 || !(fabs(a->scale) <= 1e30)) return FF_ERR_ARG;
     if (a->cache.dh != 32 && a->cache.dh != 64 && a->cache.dh != 128 && a->cache.dh != 256) return FF_ERR_UNSUPPORTED;
     if (a->H > 65535 || a->cache.B > 65535 || a->cache.n * a->H > 61439 * 16) return FF_ERR_UNSUPPORTED;      // (grids: kv heads x groups of 16 rows)
     const int64_t per = a->cache.dtype == FF_F32 ? 4 : 8;

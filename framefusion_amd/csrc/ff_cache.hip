@@ -10,11 +10,12 @@ namespace ff {
 constexpr int kRowThreads = 256;
 
 int cache_check(const ff_cache_t* c) {
-    if (!c->keys || !c->values || !c->table || !c->start) return FF_ERR_ARG;
+    // (an empty tensor may have no address: a pool of no pages, a table of no width, a batch of nothing)
+    if ((c->n_pages && (!c->keys || !c->values)) || (c->table_width && c->B && !c->table) || (c->B && !c->start)) return FF_ERR_ARG;
     if (c->dtype != FF_F32 && c->dtype != FF_BF16 && c->dtype != FF_F16) return FF_ERR_ARG;
     const bool codes = c->store == FF_STORE_E4M3 || c->store == FF_STORE_E2M1;
     if (!codes && c->store != c->dtype) return FF_ERR_ARG;
-    if (codes && (!c->key_scales || !c->value_scales)) return FF_ERR_ARG;
+    if (codes && c->n_pages && (!c->key_scales || !c->value_scales)) return FF_ERR_ARG;
     if (c->n_pages < 0 || c->kv_heads < 1 || c->page_size < 1 || c->dh < 1 || c->table_width < 0 || c->B < 0 || c->n < 0) return FF_ERR_ARG;
     if (!cache_aligned(c->keys) || !cache_aligned(c->values) || !cache_aligned(c->key_scales) || !cache_aligned(c->value_scales)) return FF_ERR_ALIGN;
     if (c->dh % 32 || c->dh > 256 || c->page_size % 16 || c->page_size > 65536 || c->n_pages > 0x7fffffff || c->kv_heads > 4096) return FF_ERR_UNSUPPORTED;

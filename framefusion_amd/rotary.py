@@ -110,6 +110,8 @@ class _Rotary(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dq, dk):
+        if torch.cuda.is_current_stream_capturing():
+            raise FrameFusionHipError("apply_rotary: a differentiable call cannot be captured into a graph (use transpose=True on the gradients)")
         cos, sin = ctx.saved_tensors
         sections, interleaved, transpose = ctx.how
         turn = _Rotary.apply if torch.is_grad_enabled() else _lib.host().rotary           # (differentiated again, or the end of the line)

@@ -413,7 +413,8 @@ int ff_rotary_apply(const ff_rotary_t* args);
  * ff_cache_write: n tokens from start[b] on.  Block scale 2^e: the smallest e with max|x| <= 448 * 2^e (e4m3) or 6 * 2^e (e2m1),
  *   e >= -100; codes round to nearest even.  |x| is first limited to 1.875 (e4m3) / 1.5 (e2m1) * 2^127 (FF_F16: 2^15), so that every
  *   stored value is finite in T; a block with a NaN or infinity is stored as NaN.
- * ff_cache_read: the values of n tokens from start[b] on, rounded once to T.
+ * ff_cache_read: the values of n tokens from start[b] on, rounded once to T (FF_F16: values written as FF_BF16 / FF_F32 may pass its
+ *   range and become infinities; the same holds for the keys and values that ff_cache_attention reads as FF_F16).
  * ff_cache_keep: row start[b] + i becomes a copy of row start[b] + accepted[b * m + i]; the list ends at the first entry that
  *   is negative, not larger than the one before, or without a place. */
 enum { FF_STORE_E2M1 = 4, FF_STORE_E4M3 = 8 };
@@ -440,7 +441,7 @@ int ff_cache_keep(const ff_cache_t* cache, const int32_t* accepted, int64_t m, f
 /* ff_cache_attention: out_i = sum_j softmax_j(scale q_i . k_j) v_j for the n new tokens of each sequence, whose keys and values
  *   lie in the cache behind its start[b] earlier ones.  Token i sees every earlier token, and new token j where
  *   mask[b * mask_batch + i * n + j] != 0 (mask = NULL: j <= i).  What it does not see contributes nothing, whatever is stored
- *   there; a token that sees nothing gets zeros.  Scores, statistics and sums in fp32; the probabilities are rounded to T before
+ *   there; a token that sees nothing gets zeros.  |scale| <= 1e30.  Scores, statistics and sums in fp32; the probabilities are rounded to T before
  *   they meet the values.  ws: ff_cache_attention_workspace_bytes(args) bytes (may be 0), not initialised, dead when the call's
  *   work is done. */
 typedef struct ff_cache_attention {

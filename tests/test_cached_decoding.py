@@ -63,7 +63,7 @@ def test_call_arguments_are_refused():
         assert lib.ff_cache_write(pack(_lib.CACHE_ROWS, CACHE, ROWS, **change)) == want
         assert lib.ff_cache_read(pack(_lib.CACHE_ROWS, CACHE, ROWS, **change)) == want
     for change, want in ((dict(q=0), ERR_ARG), (dict(out=0), ERR_ARG), (dict(H=3), ERR_ARG), (dict(H=0), ERR_ARG), (dict(mask_batch=-1), ERR_ARG),
-                         (dict(q=4104), ERR_ALIGN), (dict(q_head=4), ERR_ALIGN), (dict(dh=96), ERR_UNSUPPORTED), (dict(H=1 << 17), ERR_UNSUPPORTED)):
+                         (dict(scale=float("nan")), ERR_ARG), (dict(scale=float("-inf")), ERR_ARG), (dict(q=4104), ERR_ALIGN), (dict(q_head=4), ERR_ALIGN), (dict(dh=96), ERR_UNSUPPORTED), (dict(H=1 << 17), ERR_UNSUPPORTED)):
         assert lib.ff_cache_attention(pack(_lib.CACHE_ATTENTION, CACHE, ATT, **change)) == want
     assert lib.ff_cache_keep(pack(_lib.CACHE, CACHE), None, 2, None) == ERR_ARG
     assert lib.ff_cache_keep(pack(_lib.CACHE, CACHE), 64, -1, None) == ERR_ARG
@@ -132,6 +132,12 @@ def test_python_refusals_without_a_gpu():
         lambda: ffa.cache_write(c._replace(keys=c.keys.transpose(1, 2)), x, x, table, start),
         lambda: ffa.cache_write(cpu_cache("fp8")._replace(key_scales=None), x, x, table, start),
         lambda: ffa.cache_write(cpu_cache("fp4")._replace(value_scales=torch.zeros(1, dtype=torch.uint8)), x, x, table, start),
+        lambda: ffa.cache_write((1, 2, 3, 4), x, x, table, start),
+        lambda: ffa.cache_write(c[:3], x, x, table, start),
+        lambda: ffa.cache_write(c, None, x, table, start),
+        lambda: ffa.cache_write(c, x, x, None, start),
+        lambda: ffa.cache_read(c, table, start, 4, dtype="bf16"),
+        lambda: ffa.cache_attention(q, c, table, start, mask=3),
         lambda: ffa.cache_read(c, table, start, -1),
         lambda: ffa.cache_read(c, table, start, 4, dtype=torch.float32),
         lambda: ffa.cache_keep(c, table, start, torch.zeros(2, 3)),
@@ -148,6 +154,10 @@ def test_python_refusals_without_a_gpu():
         with pytest.raises(ffa.FrameFusionHipError):
             call()
             pytest.fail(f"call {at} was not refused")
+    with pytest.raises(TypeError):
+        ffa.cache_attention(q, c, table, start, scale="half")
+    with pytest.raises(TypeError):
+        ffa.cache_read(c, table, start, 2.5)
     # what is right but for the device says so
     for call in (lambda: ffa.cache_write(c, x, x, table, start), lambda: ffa.cache_attention(q, c, table, start),
                  lambda: ffa.cache_read(c, table, start, 4), lambda: ffa.cache_keep(c, table, start, torch.zeros(2, 3, dtype=torch.int32))):

@@ -169,6 +169,29 @@ def test_apply_rotary_under_capture():
             assert torch.equal(got, want)
 
 
+def test_backward_under_capture_is_refused(monkeypatch):
+    q, k = torch.randn(1, 4, 6, 64, device=DEV, requires_grad=True), torch.randn(1, 2, 6, 64, device=DEV)
+    cos, sin = torch.randn(1, 6, 64, device=DEV), torch.randn(1, 6, 64, device=DEV)
+    y, _ = ffa.apply_rotary(q, k, cos, sin)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(ffa.FrameFusionHipError, match="capture"):
+        torch.autograd.grad(y.sum(), q)
+
+
+def test_apply_rotary_of_expanded_inputs():
+    """One head shown to several (stride 0): the gradient of the shared one is the sum over them."""
+    one = torch.randn(2, 1, 5, 32, device=DEV, requires_grad=True)
+    k = torch.randn(2, 2, 5, 32, device=DEV)
+    cos, sin = torch.randn(1, 5, 32, device=DEV), torch.randn(1, 5, 32, device=DEV)
+    y, _ = ffa.apply_rotary(one.expand(-1, 3, -1, -1), k, cos, sin)
+    whole = one.detach().repeat(1, 3, 1, 1).requires_grad_()
+    z, _ = ffa.apply_rotary(whole, k, cos, sin)
+    assert torch.equal(y, z)
+    dy = torch.randn_like(y)
+    got, want = torch.autograd.grad(y, one, dy)[0], torch.autograd.grad(z, whole, dy)[0].double().sum(1, keepdim=True)
+    within(got, want, 4 * U * torch.autograd.grad(ffa.apply_rotary(whole, k, cos, sin)[0], whole, dy)[0].double().abs().sum(1, keepdim=True))
+
+
 # ---------------------------------------------------------------------------------------------------- the cache
 LIMIT = {"fp8": (448.0, 1.875, -6, 3), "fp4": (6.0, 1.5, 0, 1)}
 
@@ -436,6 +459,29 @@ def test_attention_types_and_heads(dtype, store, dh):
     attention_case(dtype, store, dh, 2, 4, 65, 48, [290])
 
 
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("store", ["fp8", "fp4"])
+@pytest.mark.parametrize("dh,n,G", [(32, 1, 2), (64, 3, 2), (128, 1, 7), (256, 2, 3), (64, 60, 3), (128, 61, 3), (256, 60, 3), (32, 70, 2)])
+def test_attention_over_blocks_of_nan(dtype, store, dh, n, G):
+    """A NaN that was written into the earlier tokens is one block of NaN: as a key it reaches every output of its head, as a value its own
+    32 channels; as a new token's value only those of the tokens that see it."""
+    T = DT[dtype]
+    ctx, bad = 77, 40
+    gen = torch.Generator(device=DEV).manual_seed(dh + n)
+    k, v = (torch.randn(1, 3, ctx + n, dh, generator=gen, device=DEV).to(T) for _ in range(2))
+    k[0, 0, bad, 5] = math.nan
+    v[0, 1, bad, dh - 1] = math.inf
+    v[0, 2, ctx + n - 1, 0] = math.nan
+    cache = ffa.new_cache(16, 16, 3, dh, T, store, device=DEV)
+    table, start = torch.randperm(16, generator=gen, device=DEV).to(torch.int32)[None].contiguous(), torch.tensor([ctx], dtype=torch.int32, device=DEV)
+    ffa.cache_write(cache, k, v, table, torch.zeros_like(start))
+    q = torch.randn(1, 3 * G, n, dh, generator=gen, device=DEV).to(T)
+    got = ffa.cache_attention(q, cache, table, start)[0].unflatten(0, (3, G))
+    assert torch.isnan(got[0]).all()
+    assert torch.isnan(got[1][..., dh - 32:]).all() and torch.isfinite(got[1][..., : dh - 32]).all()
+    assert torch.isfinite(got[2][:, : n - 1]).all() and torch.isfinite(got[2][..., 32:]).all() and torch.isnan(got[2][:, n - 1, :32]).all()
+
+
 def test_attention_of_infinite_values_that_only_some_see():
     """A value of infinity (its key finite): infinity for the tokens that see it, nothing for the others."""
     for dtype, n, kv, G in (("bf16", 9, 2, 3), ("bf16", 64, 1, 3), ("fp32", 9, 2, 3)):
@@ -510,6 +556,41 @@ def test_attention_scales(scale):
 @pytest.mark.parametrize("dtype,store,ctx", [("bf16", "fp4", 70001), ("bf16", None, 20011), ("fp32", None, 9001)])
 def test_attention_long(dtype, store, ctx):
     attention_case(dtype, store, 64, 1, 2, 2, 128, [ctx, ctx // 3])
+
+
+def test_empty_calls():
+    cache = ffa.new_cache(4, 16, 2, 64, torch.bfloat16, "fp8", device=DEV)
+    start = torch.zeros(2, dtype=torch.int32, device=DEV)
+    for width in (0, 2):
+        table = torch.full((2, width), -1, dtype=torch.int32, device=DEV)               # no place at all
+        x = torch.randn(2, 2, 3, 64, device=DEV).bfloat16()
+        ffa.cache_write(cache, x, x, table, start)
+        assert not any(t.view(torch.uint8).any() for t in cache)
+        assert not ffa.cache_read(cache, table, start, 3)[0].any()
+        for n in (3, 70):
+            assert not ffa.cache_attention(torch.randn(2, 4, n, 64, device=DEV).bfloat16(), cache, table, start).any()
+        ffa.cache_keep(cache, table, start, torch.tensor([[1], [2]], dtype=torch.int32, device=DEV))
+    none = ffa.new_cache(0, 16, 2, 64, torch.bfloat16, None, device=DEV)
+    table = torch.zeros(2, 3, dtype=torch.int32, device=DEV)
+    for n in (1, 70):
+        assert not ffa.cache_attention(torch.randn(2, 4, n, 64, device=DEV).bfloat16(), none, table, start).any()
+    assert ffa.cache_attention(torch.randn(2, 4, 0, 64, device=DEV).bfloat16(), cache, table, start).shape == (2, 4, 0, 64)
+    assert ffa.cache_read(cache, table, start, 0)[0].shape == (2, 2, 0, 64)
+    table, start = torch.zeros(0, 3, dtype=torch.int32, device=DEV), torch.zeros(0, dtype=torch.int32, device=DEV)
+    assert ffa.cache_attention(torch.randn(0, 4, 1, 64, device=DEV).bfloat16(), cache, table, start).shape == (0, 4, 1, 64)
+    with pytest.raises(ffa.FrameFusionHipError):
+        ffa.cache_attention(torch.randn(2, 4, 1, 64, device=DEV).bfloat16(), cache, torch.zeros(2, 3, dtype=torch.int32, device=DEV),
+                            torch.zeros(2, dtype=torch.int32, device=DEV), scale=math.nan)
+
+
+def test_many_sequences():
+    """More sequences than a wave has lanes, and than there are workgroups over the keys: ragged, padded, empty ones among them."""
+    gen = torch.Generator().manual_seed(7)
+    for B, longest, n in ((150, 300, 1), (70, 900, 3), (300, 40, 2)):
+        starts = torch.randint(-1, longest, (B,), generator=gen).tolist()
+        starts[3], starts[64] = 0, longest
+        attention_case("bf16", "fp8", 32, 1, 2, n, 16, starts)
+    attention_case("bf16", None, 32, 1, 2, 66, 16, torch.randint(-1, 200, (70,), generator=gen).tolist(), mask=None)
 
 
 def test_attention_beyond_32_bit_offsets():
