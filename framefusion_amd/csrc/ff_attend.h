@@ -78,14 +78,15 @@ __device__ inline int blocks_of(const ff_cache_t& c, const AttPlan& p, int b) { 
 __device__ inline bool share_of(const ff_cache_t& c, const AttPlan& p, int w, Share& s) {
     const int B = (int)c.B, lane = threadIdx.x & 63;
     auto sum = [&](int each) {                    // blocks of all sequences, or with each > 0 their splits of so many
-        int64_t x = 0;
+        uint32_t low = 0, high = 0;               // (2^16 sequences of 2^25 blocks pass 32 bits)
         for (int b = lane; b < B; b += 64) {
-            const int n = blocks_of(c, p, b);
-            x += each ? max(1, (n + each - 1) / each) : n;
+            const uint32_t n = blocks_of(c, p, b), x = each ? max(1u, (n + each - 1) / each) : n;
+            low += x & 0xffffu;
+            high += x >> 16;
         }
-#pragma unroll
-        for (int k = 32; k > 0; k >>= 1) x += __shfl_xor(x, k, 64);
-        return x;
+        // on the DPP network: a sum by shuffles through the LDS crossbar costs 0.5 us, and there are several
+        return (int64_t)(uint32_t)__builtin_amdgcn_readlane(wave_incl_scan_dpp((int)low), 63) +
+               ((int64_t)(uint32_t)__builtin_amdgcn_readlane(wave_incl_scan_dpp((int)high), 63) << 16);
     };
     const int64_t total = sum(0);
     int each = (int)max((int64_t)1, (total + p.want - 1) / p.want);
