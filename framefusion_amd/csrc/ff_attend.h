@@ -62,6 +62,10 @@ struct AttPlan {                    // what the host derives once a call
     int64_t part_rows;
 };
 
+// Weights are 2^(score - maximum + lift), which leaves sums and outputs scaled alike.  fp16 keeps numbers from 2^-14 whole: with the maximum
+// allowed to lag by 2^8, a lift of 2^7 still fits (2^15), and weights down to 2^-21 of the largest lose nothing (2^-32: are not lost).
+template <int DT> constexpr float kLift = DT == FF_F16 ? 7.f : 0.f;
+
 // keys of a sequence that the new tokens may see: everything before them and themselves, as far as the table reaches
 __device__ inline int64_t keys_of(const ff_cache_t& c, int64_t start) {
     const int64_t room = c.n_pages > 0 ? c.table_width * c.page_size : 0;

@@ -197,7 +197,16 @@ template <int DT, int STORE, int DH> __device__ inline bool take_out_odd(Raw<DT,
 #pragma unroll
         for (int y = 0; y < G::kVW; ++y) {
             uint32_t& w = raw.v[j][y];
-            if constexpr (STORE == FF_STORE_E4M3) {                 // the code of all ones is NaN
+            if constexpr (G::kCodes && DT == FF_F16) {              // (values written as another type may pass fp16's range)
+                constexpr int kPer = STORE == FF_STORE_E4M3 ? 2 : 4, kWidth = 16 / kPer;
+                const float scale = __uint_as_float(value_scale<DT, STORE, DH>(raw, j, lane) << 23);
+#pragma unroll
+                for (int k = 0; k < kPer; ++k) {
+                    const uint32_t pair = codes2<DT, STORE>(w, scale, k);
+                    if ((pair & 0x7c00u) == 0x7c00u) w &= ~(((1u << kWidth) - 1) << (2 * k * kWidth)), odd = true;
+                    if ((pair & 0x7c000000u) == 0x7c000000u) w &= ~(((1u << kWidth) - 1) << ((2 * k + 1) * kWidth)), odd = true;
+                }
+            } else if constexpr (STORE == FF_STORE_E4M3) {                 // the code of all ones is NaN
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                     if (((w >> (8 * k)) & 0x7fu) == 0x7fu) w &= ~(255u << (8 * k)), odd = true;
@@ -365,7 +374,7 @@ __global__ __launch_bounds__(64 * kAttWaves, DH * NT * (STORE == kStoreSame ? Ac
 #pragma unroll
                 for (int y = 0; y < kTiles; ++y) o[t][y] *= down;
             }
-            const float zero = m[t] == kNone ? 0.f : m[t];
+            const float zero = (m[t] == kNone ? 0.f : m[t]) - kLift<DT>;
             float sum = 0.f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {

@@ -274,7 +274,7 @@ __global__ __launch_bounds__(64 * NW, DH == 256 ? 1 : 2) void k_cache_attention_
 #pragma unroll
                     for (int y = 0; y < kTiles; ++y) o[y] *= down;
                 }
-                const float zero = m == kNone ? 0.f : m;
+                const float zero = (m == kNone ? 0.f : m) - kLift<DT>;
                 float sum = 0.f;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
@@ -369,7 +369,7 @@ __global__ __launch_bounds__(64 * NW, DH == 256 ? 1 : 2) void k_cache_attention_
 template <int DT, int STORE, int DH, int NW>
 static int launch_rows_of(const ff_cache_attention_t* a, const AttPlan& p) {
     constexpr int kBytes = 4 * kRowsKeys * DH * 2 + (DH <= 128 ? NW * 64 * DH : 0);           // two buffers, and Q
-    static_assert(kBytes + 64 <= 160 * 1024, "two buffers fit the shared memory of a CU");
+    static_assert(kBytes + 2 * 32 * NW * 8 + 64 <= 160 * 1024, "two buffers, Q and the rest fit the shared memory of a CU");
     static std::atomic<bool> ready[kMaxDevices];
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= kMaxDevices) dev = -1;
@@ -380,6 +380,7 @@ static int launch_rows_of(const ff_cache_attention_t* a, const AttPlan& p) {
     }
     const ff_cache_t& c = a->cache;
     const int64_t across = c.kv_heads * (p.slots == 1 ? c.B : p.slots);
+    if ((across + 7) / 8 * 8 * p.groups > 0x7fffffff) return FF_ERR_UNSUPPORTED;
     const dim3 grid((uint32_t)((across + 7) / 8 * 8 * p.groups));
     k_cache_attention_rows<DT, STORE, DH, NW><<<grid, 64 * NW, kBytes, (hipStream_t)a->stream>>>(*a, p);
     return (int)hipGetLastError();

@@ -583,6 +583,51 @@ def test_empty_calls():
                             torch.zeros(2, dtype=torch.int32, device=DEV), scale=math.nan)
 
 
+@pytest.mark.parametrize("n,G", [(1, 2), (70, 2)])
+@pytest.mark.parametrize("first", [True, False])
+def test_attention_small_weights_in_fp16(n, G, first):
+    """One key with nearly all the weight and 20 000 others of 2^-23 to 2^-27 of it each, whose values are what comes out.  A weight keeps
+    2^-12 of itself, or what lies 2^-32 below the largest: rounded to fp16 as it stands it would be off by 2^-25."""
+    dh, ctx = 64, 20000
+    gen = torch.Generator(device=DEV).manual_seed(n)
+    k, v = torch.zeros(1, 1, ctx + n, dh, device=DEV), torch.zeros(1, 1, ctx + n, dh, device=DEV)
+    top = 0 if first else ctx - 1
+    k[..., 0] = -(23 + 4 * torch.rand(ctx + n, generator=gen, device=DEV))             # score in octaves below the top one's 0
+    v[:] = 500 + 100 * torch.randn(v.shape, generator=gen, device=DEV)
+    k[0, 0, top], v[0, 0, top] = 0, 0
+    k, v = k.half(), v.half()
+    cache = ffa.new_cache(160, 128, 1, dh, torch.float16, None, device=DEV)
+    table, start = torch.arange(160, dtype=torch.int32, device=DEV)[None], torch.tensor([ctx], dtype=torch.int32, device=DEV)
+    ffa.cache_write(cache, k, v, table, torch.zeros_like(start))
+    q = torch.zeros(1, G, n, dh, device=DEV).half()
+    q[..., 0] = 1
+    got = ffa.cache_attention(q, cache, table, start, scale=math.log(2))
+    x = k[0, 0, :, 0].double() * math.log(2)
+    for i in (0, n - 1):
+        p = torch.softmax(x[: ctx + i + 1], 0)
+        want = p @ v[0, 0, : ctx + i + 1].double()
+        tol = (p @ v[0, 0, : ctx + i + 1].double().abs()) * (half_step(torch.float16) + (ctx + n + 200) * U) + (ctx + n) * 2.0 ** -33 * 1000
+        for g in range(G):
+            within(got[0, g, i], want, tol + rounding(torch.float16, want))
+
+
+@pytest.mark.parametrize("store", ["fp8", "fp4"])
+@pytest.mark.parametrize("n", [3, 130])
+def test_fp16_attention_over_values_beyond_its_range(store, n):
+    """A cache written as bf16 and read as fp16: a value that passes fp16's range is an infinity for the tokens that see it, and nothing to
+    the others."""
+    cache = ffa.new_cache(16, 16, 1, 64, torch.bfloat16, store, device=DEV)
+    table, start = torch.arange(16, dtype=torch.int32, device=DEV)[None], torch.tensor([20], dtype=torch.int32, device=DEV)
+    k, v = (torch.randn(1, 1, 20 + n, 64, device=DEV).bfloat16() for _ in range(2))
+    v[0, 0, 21, 5], v[0, 0, 21, 6] = 3e6, -3e6
+    ffa.cache_write(cache, k, v, table, torch.zeros_like(start))
+    q = torch.randn(1, 1, n, 64, device=DEV).half()
+    got = ffa.cache_attention(q, cache, table, start, mask=torch.eye(n, dtype=torch.bool, device=DEV))[0, 0]
+    assert got[1, 5] == math.inf and got[1, 6] == -math.inf
+    got[1, 5:7] = 0
+    assert torch.isfinite(got).all()
+
+
 def test_many_sequences():
     """More sequences than a wave has lanes, and than there are workgroups over the keys: ragged, padded, empty ones among them."""
     gen = torch.Generator().manual_seed(7)
