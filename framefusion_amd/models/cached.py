@@ -28,6 +28,15 @@ def position_tables(model, cache, hidden_states, position_ids, attention_mask, t
     return list(rotary_tables(position_ids.contiguous(), rotary.inv_freq.double(), dtype=hidden_states.dtype, factor=rotary.attention_scaling))
 
 
+def prefill_mask(model, cache, hidden_states):
+    """The causal mask of a prefill's own attention, in the form that the configured attention asks for (None where it is causal by
+    itself).  A step has none: ``cache_attention`` masks by position or by ``tree_mask``."""
+    from transformers.masking_utils import create_causal_mask
+    if cache.get_seq_length():
+        return None
+    return create_causal_mask(config=model.config, inputs_embeds=hidden_states, attention_mask=None, past_key_values=None, position_ids=None)
+
+
 def rotate(query_states, key_states, cos, sin, sections=None):
     return apply_rotary(query_states, key_states, cos, sin, sections=sections)
 

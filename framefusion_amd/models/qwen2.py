@@ -24,7 +24,7 @@ from ..cache import ReducedCache
 from ..interface import Family, register_family
 from ..main import call_b_with_residual
 from ..utils import last_query_importance
-from .cached import cached_attention, continues, finish_step, position_tables, rotate
+from .cached import cached_attention, continues, finish_step, position_tables, prefill_mask, rotate
 
 
 def qwen2_attention_forward(self, hidden_states, position_embeddings, attention_mask, past_key_values=None, tree_mask=None, **kwargs):
@@ -103,9 +103,9 @@ def qwen2_model_forward(self, input_ids=None, attention_mask=None, position_ids=
         position_ids = (torch.arange(inputs_embeds.shape[1], device=inputs_embeds.device) + seen).unsqueeze(0)
     hidden_states = inputs_embeds
     if isinstance(past_key_values, ReducedCache):
-        causal_mask = None
         position_embeddings = position_tables(self, past_key_values, hidden_states, position_ids, attention_mask,
                                               kwargs.get("tree_mask"))
+        causal_mask = prefill_mask(self, past_key_values, hidden_states)
     else:
         causal_mask = create_causal_mask(config=self.config, inputs_embeds=inputs_embeds, attention_mask=attention_mask,
                                          past_key_values=past_key_values, position_ids=position_ids)

@@ -23,7 +23,7 @@ from ..cache import ReducedCache
 from ..interface import Family, register_family
 from ..main import call_b_with_residual
 from ..utils import last_query_importance
-from .cached import cached_attention, continues, finish_step, position_tables, rotate
+from .cached import cached_attention, continues, finish_step, position_tables, prefill_mask, rotate
 
 NUM_IMPORTANCE_QUERIES = 4           # modeling_qwen2_vl.py:296
 
@@ -109,9 +109,9 @@ def qwen2vl_text_model_forward(self, input_ids=None, attention_mask=None, positi
         text_position_ids, position_ids = position_ids[0], position_ids[1:]
     hidden_states = inputs_embeds
     if isinstance(past_key_values, ReducedCache):
-        causal_mask = None
         position_embeddings = position_tables(self, past_key_values, hidden_states, position_ids, attention_mask,
                                               kwargs.get("tree_mask"))
+        causal_mask = prefill_mask(self, past_key_values, hidden_states)
     else:
         causal_mask = create_causal_mask(config=self.config, inputs_embeds=inputs_embeds, attention_mask=attention_mask,
                                          past_key_values=past_key_values, position_ids=text_position_ids)

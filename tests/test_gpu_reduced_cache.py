@@ -113,6 +113,25 @@ def test_prefill_tokens_and_trees(family):
         close(prefill(model, new, emb, pt), prefill(model, DynamicCache(config=cfg), emb, pt))
 
 
+@pytest.mark.parametrize("family", ["qwen2", "qwen2_vl"])
+def test_attention_that_needs_a_mask(family):
+    """Eager attention is causal only by its mask: the prefill gets one, with a ReducedCache as with a DynamicCache."""
+    from transformers.cache_utils import DynamicCache
+    model, cfg = (qwen2 if family == "qwen2" else qwen2_vl)()
+    emb, pt = video_tokens(F_, P, D, p_change=0.5, sigma=0.3, sigma_hi=1.2, seed=11, pre=PRE, post=POST, dtype=torch.float32)
+    emb = emb.to(DEV)
+    L = emb.shape[1]
+    cfg._attn_implementation = "eager"
+    old, new = DynamicCache(config=cfg), ffa.ReducedCache(4, 2, 32, 512, dtype=torch.float32, device=DEV)
+    with torch.no_grad():
+        close(prefill(model, new, emb, pt), prefill(model, old, emb, pt))
+        x = torch.randn(1, 1, D, generator=torch.Generator(device=DEV).manual_seed(2), device=DEV)
+        step = [dict(inputs_embeds=x, past_key_values=c, use_cache=True, position_ids=positions(family, [L])) for c in (new, old)]
+        got = model.model(**step[0]).last_hidden_state
+        cfg._attn_implementation = "sdpa"              # (a step's eager mask has layer 0's length, a DynamicCache another in every layer)
+        close(got, model.model(**step[1]).last_hidden_state)
+
+
 @pytest.mark.parametrize("store", ["fp8", "fp4", None])
 def test_quantised_cache_runs(store):
     """bf16 model, keys and values in 8 and 4 bits: what is stored is the rounding of what a cache in bf16 holds (fp32 of it against the
