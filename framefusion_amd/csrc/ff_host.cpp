@@ -78,11 +78,10 @@ struct Cache {
 
 // the head of every call on a cache: (keys, values, key_scales, value_scales), its table and start
 Cache parse(PyObject* cache, PyObject* table_o, PyObject* start_o, int64_t n, at::ScalarType dtype, const char* what) {
-    PyObject* seq = PySequence_Fast(cache, "a cache is the four tensors (keys, values, key_scales, value_scales)");
-    if (!seq) throw python_error();
-    struct Release { PyObject* p; ~Release() { Py_DECREF(p); } } release{seq};
-    if (PySequence_Fast_GET_SIZE(seq) != 4) refuse(what, ": a cache is the four tensors (keys, values, key_scales, value_scales)");
-    PyObject** items = PySequence_Fast_ITEMS(seq);
+    // (the caller's own tuple holds the tensors while the call runs: what an iterator made would be gone before the launch)
+    if (!(PyTuple_Check(cache) || PyList_Check(cache)) || PySequence_Fast_GET_SIZE(cache) != 4)
+        refuse(what, ": a cache is the four tensors (keys, values, key_scales, value_scales)");
+    PyObject** items = PySequence_Fast_ITEMS(cache);
     const at::Tensor &keys = tensor(items[0], what, "keys"), &values = tensor(items[1], what, "values");
     Cache out;
     out.device = keys.device();
@@ -265,7 +264,7 @@ PyObject* py_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     }
     Cache cache = parse(args[1], args[2], args[3], n, query.scalar_type(), what);
     const ff_cache_t& c = cache.c;
-    if (B != c.B || dh != c.dh || H < 1 || H % c.kv_heads || query.device() != cache.device)
+    if (B != c.B || dh != c.dh || H < 1 || c.kv_heads < 1 || H % c.kv_heads || query.device() != cache.device)
         refuse("cache_attention: query ", query.sizes(), " does not fit a table of ", c.B, " sequences and ", c.kv_heads, " heads of ", c.dh);
     const c10::DeviceGuard guard(cache.device);
     const at::Tensor out = at::empty({B, n, H, dh}, query.options());

@@ -165,6 +165,18 @@ def test_python_refusals_without_a_gpu():
             call()
 
 
+def test_a_cache_is_a_tuple_or_a_list():
+    """The tensors of an iterator would be gone before the launch."""
+    x, table, start = torch.zeros(2, 2, 5, 64), torch.zeros(2, 3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    c = cpu_cache(dtype=torch.float32, dh=64)
+    for cache in (iter(c), (t for t in c), {t: 0 for t in range(4)}, None):
+        with pytest.raises(ffa.FrameFusionHipError, match="four tensors"):
+            ffa.cache_write(cache, x, x, table, start)
+    for cache in (c, list(c), tuple(c)):
+        with pytest.raises(ffa.FrameFusionHipError, match="MI355X only"):
+            ffa.cache_write(cache, x, x, table, start)
+
+
 def test_rotary_refusals_without_a_gpu():
     q, k = torch.zeros(1, 4, 5, 32), torch.zeros(1, 2, 5, 32)
     t, t3 = torch.zeros(1, 5, 32), torch.zeros(3, 1, 5, 32)

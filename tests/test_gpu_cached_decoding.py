@@ -583,6 +583,15 @@ def test_empty_calls():
                             torch.zeros(2, dtype=torch.int32, device=DEV), scale=math.nan)
 
 
+def test_cache_without_heads_is_refused():
+    x = torch.zeros(2, 0, 16, 64, device=DEV).bfloat16()
+    table, start = torch.zeros(1, 2, dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    with pytest.raises(ffa.FrameFusionHipError, match="0 heads"):
+        ffa.cache_attention(torch.randn(1, 4, 1, 64, device=DEV).bfloat16(), (x, x, None, None), table, start)
+    with pytest.raises(ffa.FrameFusionHipError):
+        ffa.cache_keep((x, x, None, None), table, start, torch.ones(1, 1, dtype=torch.int32, device=DEV))
+
+
 @pytest.mark.parametrize("n,G", [(1, 2), (70, 2)])
 @pytest.mark.parametrize("first", [True, False])
 def test_attention_small_weights_in_fp16(n, G, first):
