@@ -220,10 +220,18 @@ template <int DT, int STORE, int DH> __device__ inline bool take_out_odd(Raw<DT,
     return odd;
 }
 
+// Registers: keys and values of two steps (one in use, one on its way), Q and the outputs.  Where they pass 256 the kernel runs one wave a
+// SIMD with 512 (one token of 28 / 4 fp32 heads of 128 over 8 x 20 000 keys: 257 us spilling, 148 us so); fp32 rows of 256 channels
+// pass 512 too and are loaded when they are needed (587 us spilling, 269 us so): 64 KB a wave in flight are enough for the memory.
+constexpr int waves_a_simd(int dt, int store, int dh, int nt) {
+    const int bytes = store == kStoreSame && dt == FF_F32 ? 4 : 2;
+    return dh * nt * bytes > 512 || dh == 256 || (bytes == 4 && dh == 128) ? 1 : 2;
+}
 template <int DT, int STORE, int DH, int NT>
-__global__ __launch_bounds__(64 * kAttWaves, DH * NT * (STORE == kStoreSame ? Act<DT>::kBytes : 2) > 512 || DH == 256 ? 1 : 2) void k_cache_attention(const ff_cache_attention_t a, const AttPlan p) {
+__global__ __launch_bounds__(64 * kAttWaves, waves_a_simd(DT, STORE, DH, NT)) void k_cache_attention(const ff_cache_attention_t a, const AttPlan p) {
     using G = Geo<DT, STORE, DH>;
     constexpr int kSteps = DH / 32, kTiles = DH / 16, kPad = 4;
+    constexpr bool kAhead = !(DT == FF_F32 && STORE == kStoreSame && DH == 256);
     __shared__ float s_o[kAttWaves][16][DH + kPad];
     __shared__ float s_m[kAttWaves][16], s_l[kAttWaves][16];
     const ff_cache_t& c = a.cache;
@@ -306,15 +314,19 @@ __global__ __launch_bounds__(64 * kAttWaves, DH * NT * (STORE == kStoreSame ? Ac
     if (plain && p.slots > 1) share.used = max(1, min(p.want, blocks_of(c, p, b)));
     if (split >= share.used) return;
     const int64_t stride = (int64_t)share.used * kAttWaves * kAttTile;
-    if (begin < end) {
+    if (kAhead && begin < end) {
         fetch(begin);
         look_up(begin + stride);
     }
     for (int64_t base = begin; base < end; base += stride) {
+        if constexpr (!kAhead) {
+            fetch(base);
+            look_up(base + stride);
+        }
         Raw<DT, STORE, DH> raw = next;
         const int64_t row0 = next0, row1 = next1;
         const bool have0 = row0 >= 0, have1 = row1 >= 0;
-        if (base + stride < end) {
+        if (kAhead && base + stride < end) {
             fetch(base + stride);
             look_up(base + 2 * stride);
         }
