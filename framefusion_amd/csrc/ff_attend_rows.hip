@@ -294,17 +294,20 @@ __global__ __launch_bounds__(64 * NW, DH == 256 ? 1 : 2) void k_cache_attention_
                         o[y] = mma32<DT>(make_uint4(vf[k][y][0].x, vf[k][y][0].y, vf[k][y][1].x, vf[k][y][1].y), pf[k], o[y]);
             };
             // values are read while the weights that meet them are made, and the first half's products run under the second half's
-            // softmax; the barriers keep the compiler from undoing that
+            // softmax; the barriers keep the compiler from undoing that.  (256 channels: the outputs and Q leave no registers for it - 64 new
+            // tokens of 28 / 4 heads over 8 x 20 000 keys 920 us spilling, 709 us with the values read behind the weights)
             score();
             __builtin_amdgcn_sched_barrier(0);
-            load_values(0);
+            if constexpr (kShared) load_values(0);
             __builtin_amdgcn_sched_barrier(0);
             weigh(0);
+            if constexpr (!kShared) load_values(0);
             gather();
             __builtin_amdgcn_sched_barrier(0);
-            load_values(1);
+            if constexpr (kShared) load_values(1);
             __builtin_amdgcn_sched_barrier(0);
             weigh(1);
+            if constexpr (!kShared) load_values(1);
             gather();
         }
         if (more) {
