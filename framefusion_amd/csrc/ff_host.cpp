@@ -52,7 +52,8 @@ const at::Tensor& tensor(PyObject* o, const char* what, const char* name) {
     if (!THPVariable_Check(o)) refuse(what, ": ", name, " must be a tensor");
     return THPVariable_Unpack(o);
 }
-bool differentiable(const at::Tensor& t) { return t.requires_grad() && c10::GradMode::is_enabled(); }
+// whether a derivative is asked for with respect to `t`, backward or (a tangent beside it) forward
+bool differentiable(const at::Tensor& t) { return (t.requires_grad() && c10::GradMode::is_enabled()) || t._fw_grad(0).defined(); }
 
 int code_of(at::ScalarType t) {
     switch (t) {
@@ -93,6 +94,7 @@ Cache parse(PyObject* cache, PyObject* table_o, PyObject* start_o, int64_t n, at
     if (store < 0 || keys.dim() != 4 || values.sizes() != keys.sizes() || values.scalar_type() != out.own || values.device() != out.device ||
         !keys.is_contiguous() || !values.is_contiguous())
         refuse(what, ": keys and values of a cache must be alike and contiguous, [pages, kv_heads, page_size, head_dim]");
+    if (differentiable(keys) || differentiable(values)) refuse(what, " has no gradient (serving only): call it under torch.no_grad()");
     if (code < 0) refuse(what, ": a cache serves float32, bfloat16 and float16, not ", c10::toString(dtype));
     ff_cache_t& c = out.c;
     c.n_pages = keys.size(0);
@@ -340,7 +342,9 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     a.rot = cos.size(-1);
     if ((cos.size(-3) != 1 && cos.size(-3) != a.B) || cos.size(-2) != a.L || a.rot % 2 || a.rot < 2 || a.rot > a.dh)
         refuse("apply_rotary: tables ", cos.sizes(), " do not fit query ", query.sizes());
-    if (cos.requires_grad() || sin.requires_grad()) refuse("apply_rotary: the tables are constants, they have no gradient");
+    if (cos.requires_grad() || sin.requires_grad() || differentiable(cos) || differentiable(sin))
+        refuse("apply_rotary: the tables are constants, they have no gradient");
+    if (query._fw_grad(0).defined() || key._fw_grad(0).defined()) refuse("apply_rotary: tangents go through the autograd function");
     on_gpu(query, what);
     const c10::DeviceGuard guard(device);
     const at::AutoDispatchBelowADInplaceOrView below;          // (the caller has dealt with autograd)

@@ -9,6 +9,7 @@ import math
 from typing import Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import FrameFusionHipError
@@ -71,6 +72,11 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: Optional[dict] 
     raise FrameFusionHipError(f"rotary scaling {kind!r} is not one of default, linear, ntk, yarn, llama3")
 
 
+def _has_tangent(*tensors) -> bool:
+    """Whether forward-mode differentiation asks for a derivative with respect to one of them."""
+    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def rotary_tables(positions: torch.Tensor, inv_freq: torch.Tensor, dtype: torch.dtype = torch.bfloat16, factor: float = 1.0,
                   interleaved: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
     """(cos, sin) of shape ``positions.shape + (2 * len(inv_freq),)``: int64 positions [B, L] or, one row an axis, [3, B, L];
@@ -81,7 +87,7 @@ def rotary_tables(positions: torch.Tensor, inv_freq: torch.Tensor, dtype: torch.
     code = _CODE.get(dtype)
     if code is None:
         raise FrameFusionHipError(f"rotary_tables: dtype {dtype} is not float32, bfloat16 or float16")
-    if positions.requires_grad or inv_freq.requires_grad:
+    if positions.requires_grad or inv_freq.requires_grad or _has_tangent(inv_freq):
         raise FrameFusionHipError("rotary_tables has no gradient")
     if dev.type != "cuda":
         _lib.require_gpu(positions, "rotary_tables")
@@ -100,23 +106,30 @@ def rotary_tables(positions: torch.Tensor, inv_freq: torch.Tensor, dtype: torch.
 
 
 class _Rotary(torch.autograd.Function):
-    """y = R x for both inputs; the gradient is R^T (itself a rotation call, so it can be differentiated again)."""
+    """y = R x for both inputs; the gradient is R^T, the tangent R (rotation calls themselves, so they can be differentiated again)."""
 
     @staticmethod
     def forward(ctx, query, key, cos, sin, sections, interleaved, transpose):
         ctx.save_for_backward(cos, sin)
+        ctx.save_for_forward(cos, sin)
         ctx.how = (sections, interleaved, transpose)
         return _lib.host().rotary(query, key, cos, sin, sections, interleaved, transpose)
 
     @staticmethod
     def backward(ctx, dq, dk):
-        if torch.cuda.is_current_stream_capturing():
+        if dq.is_cuda and torch.cuda.is_current_stream_capturing():
             raise FrameFusionHipError("apply_rotary: a differentiable call cannot be captured into a graph (use transpose=True on the gradients)")
         cos, sin = ctx.saved_tensors
         sections, interleaved, transpose = ctx.how
         turn = _Rotary.apply if torch.is_grad_enabled() else _lib.host().rotary           # (differentiated again, or the end of the line)
         dq, dk = turn(dq, dk, cos, sin, sections, interleaved, not transpose)
         return dq, dk, None, None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, dq, dk, *constants):
+        cos, sin = ctx.saved_tensors
+        sections, interleaved, transpose = ctx.how
+        return apply_rotary(dq, dk, cos, sin, sections, interleaved, transpose)
 
 
 def apply_rotary(query: torch.Tensor, key: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, sections: Optional[Sequence[int]] = None,
@@ -126,9 +139,11 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor, cos: torch.Tensor, sin:
     layout: pair (i, i + rot / 2); ``interleaved``: (2i, 2i + 1).  fp32 inside, one rounding to the inputs' type.  Tables: the
     inputs' type or float32.  ``transpose`` applies the transposed rotation - the gradient, without autograd.
 
-    Differentiable in query and key (the tables are constants).  A differentiable call is not captured into a graph: capture
+    Differentiable in query and key, backward and forward (the tables are constants).  A differentiable call is not captured into a graph: capture
     ``transpose=True`` calls on the gradients instead."""
-    if (query.requires_grad or key.requires_grad) and torch.is_grad_enabled():
+    if (query.requires_grad or key.requires_grad) and torch.is_grad_enabled() or _has_tangent(query, key):
+        if _has_tangent(cos, sin):
+            raise FrameFusionHipError("apply_rotary: the tables are constants, they have no gradient")
         if query.is_cuda and torch.cuda.is_current_stream_capturing():
             raise FrameFusionHipError("apply_rotary: a differentiable call cannot be captured into a graph (use transpose=True on the gradients)")
         return _Rotary.apply(query, key, cos, sin, sections, interleaved, transpose)
