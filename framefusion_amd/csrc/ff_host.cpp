@@ -48,9 +48,18 @@ void check(int rc, const char* what) {
     }                                                     \
     END_HANDLE_TH_ERRORS
 
-const at::Tensor& tensor(PyObject* o, const char* what, const char* name) {
+// (its values lie in its memory: a sign that PyTorch keeps beside it, zeros that have none, are made so)
+at::Tensor tensor(PyObject* o, const char* what, const char* name) {
     if (!THPVariable_Check(o)) refuse(what, ": ", name, " must be a tensor");
-    return THPVariable_Unpack(o);
+    const at::Tensor& t = THPVariable_Unpack(o);
+    return t.is_neg() ? t.resolve_neg() : t._is_zerotensor() ? t.clone() : t;
+}
+// what is written in place, or read where it lies
+const at::Tensor& held(PyObject* o, const char* what, const char* name) {
+    if (!THPVariable_Check(o)) refuse(what, ": ", name, " must be a tensor");
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (t.is_neg() || t._is_zerotensor()) refuse(what, ": ", name, " must be a tensor of values that lie in memory (no negative bit, no zeros without memory)");
+    return t;
 }
 // whether a derivative is asked for with respect to `t`, backward or (a tangent beside it) forward
 bool differentiable(const at::Tensor& t) { return (t.requires_grad() && c10::GradMode::is_enabled()) || t._fw_grad(0).defined(); }
@@ -75,6 +84,7 @@ struct Cache {
     ff_cache_t c{};
     at::Device device{at::kCPU};
     at::ScalarType own;                      // of the keys
+    at::Tensor table, start;
 };
 
 // the head of every call on a cache: (keys, values, key_scales, value_scales), its table and start
@@ -83,7 +93,7 @@ Cache parse(PyObject* cache, PyObject* table_o, PyObject* start_o, int64_t n, at
     if (!(PyTuple_Check(cache) || PyList_Check(cache)) || PySequence_Fast_GET_SIZE(cache) != 4)
         refuse(what, ": a cache is the four tensors (keys, values, key_scales, value_scales)");
     PyObject** items = PySequence_Fast_ITEMS(cache);
-    const at::Tensor &keys = tensor(items[0], what, "keys"), &values = tensor(items[1], what, "values");
+    const at::Tensor &keys = held(items[0], what, "keys"), &values = held(items[1], what, "values");
     Cache out;
     out.device = keys.device();
     out.own = keys.scalar_type();
@@ -111,7 +121,7 @@ Cache parse(PyObject* cache, PyObject* table_o, PyObject* start_o, int64_t n, at
         uint8_t* scales[2];
         for (int i = 0; i < 2; ++i) {
             if (!THPVariable_Check(items[2 + i])) refuse(what, ": a cache of codes needs its scales");
-            const at::Tensor& s = THPVariable_Unpack(items[2 + i]);
+            const at::Tensor& s = held(items[2 + i], what, "scales");
             if (s.sizes() != at::IntArrayRef(want, 4) || s.scalar_type() != at::kByte || !s.is_contiguous() || s.device() != out.device)
                 refuse(what, ": a cache of codes needs contiguous uint8 scales ", at::IntArrayRef(want, 4));
             scales[i] = (uint8_t*)s.data_ptr();
@@ -119,7 +129,7 @@ Cache parse(PyObject* cache, PyObject* table_o, PyObject* start_o, int64_t n, at
         c.key_scales = scales[0];
         c.value_scales = scales[1];
     }
-    const at::Tensor &table = tensor(table_o, what, "table"), &start = tensor(start_o, what, "start");
+    const at::Tensor &table = out.table = tensor(table_o, what, "table"), &start = out.start = tensor(start_o, what, "start");
     if (table.dim() != 2 || table.scalar_type() != at::kInt || start.dim() != 1 || start.scalar_type() != at::kInt || start.size(0) != table.size(0) ||
         table.device() != out.device || start.device() != out.device || !table.is_contiguous() || !start.is_contiguous())
         refuse(what, ": table must be int32 [B, width] and start int32 [B], contiguous, on the cache's device");
@@ -159,7 +169,7 @@ void count_args(Py_ssize_t n, Py_ssize_t want, const char* what) {
 PyObject* py_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     FF_CALL
     count_args(nargs, 5, "cache_write");
-    const at::Tensor &key = tensor(args[1], "cache_write", "key"), &value = tensor(args[2], "cache_write", "value");
+    const at::Tensor key = tensor(args[1], "cache_write", "key"), value = tensor(args[2], "cache_write", "value");
     if (differentiable(key) || differentiable(value)) refuse("cache_write has no gradient (serving only): call it under torch.no_grad()");
     Cache cache = parse(args[0], args[3], args[4], key.dim() == 4 ? key.size(2) : 0, key.scalar_type(), "cache_write");
     const ff_cache_t& c = cache.c;
@@ -230,7 +240,7 @@ PyObject* py_keep(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     Py_DECREF(first);
     if (code_of(dtype) < 0) dtype = at::kBFloat16;
     Cache cache = parse(args[0], args[1], args[2], 0, dtype, "cache_keep");
-    const at::Tensor& accepted = tensor(args[3], "cache_keep", "accepted");
+    const at::Tensor accepted = tensor(args[3], "cache_keep", "accepted");
     if (accepted.scalar_type() != at::kInt || accepted.dim() != 2 || accepted.size(0) != cache.c.B || accepted.device() != cache.device ||
         !accepted.is_contiguous())
         refuse("cache_keep: accepted must be a contiguous int32 [B, m] on the cache's device");
@@ -246,7 +256,7 @@ PyObject* py_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     FF_CALL
     const char* what = "cache_attention";
     count_args(nargs, 6, what);
-    const at::Tensor& query = tensor(args[0], what, "query");
+    const at::Tensor query = tensor(args[0], what, "query");
     if (differentiable(query)) refuse("cache_attention has no gradient (serving only): call it under torch.no_grad()");
     if (query.dim() != 4) refuse("cache_attention: query must be [B, H, n, head_dim], got ", query.sizes());
     const int64_t B = query.size(0), H = query.size(1), n = query.size(2), dh = query.size(3);

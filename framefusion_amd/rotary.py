@@ -94,7 +94,7 @@ def rotary_tables(positions: torch.Tensor, inv_freq: torch.Tensor, dtype: torch.
     if dev.index != _get_device():
         with torch.cuda.device(dev):
             return rotary_tables(positions, inv_freq, dtype, factor, interleaved)
-    positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
+    positions, inv_freq = positions.resolve_neg().contiguous(), inv_freq.resolve_neg().contiguous()
     half = inv_freq.shape[0]
     both = inv_freq.new_empty((2,) + positions.shape + (2 * half,), dtype=dtype)
     cos, sin = both.select(0, 0), both.select(0, 1)

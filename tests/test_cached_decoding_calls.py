@@ -86,3 +86,16 @@ def test_what_has_no_gradient_refuses_tangents_and_caches_that_want_one():
             call()
         with torch.no_grad(), pytest.raises(ffa.FrameFusionHipError, match="MI355X only"):
             call()
+
+
+# ---- values that PyTorch keeps beside the memory
+def test_a_cache_lies_in_memory():
+    cache, x, q, table, start = cache_and_rows("fp8")
+    for bad in (cache._replace(key_scales=torch._neg_view(cache.key_scales)), cache._replace(value_scales=torch._efficientzerotensor(cache.value_scales.shape, dtype=torch.uint8))):
+        with pytest.raises(ffa.FrameFusionHipError, match="in memory"):
+            ffa.cache_write(bad, x, x, table, start)
+    cache, x, q, table, start = cache_and_rows()
+    for bad in (cache._replace(keys=torch._neg_view(cache.keys)), cache._replace(values=torch._efficientzerotensor(cache.values.shape, dtype=torch.bfloat16))):
+        for call in (lambda: ffa.cache_write(bad, x, x, table, start), lambda: ffa.cache_attention(q, bad, table, start), lambda: ffa.cache_read(bad, table, start, 2)):
+            with pytest.raises(ffa.FrameFusionHipError, match="in memory"):
+                call()
