@@ -9,10 +9,12 @@
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <cmath>
 #include <sstream>
@@ -52,7 +54,10 @@ void check(int rc, const char* what) {
 at::Tensor tensor(PyObject* o, const char* what, const char* name) {
     if (!THPVariable_Check(o)) refuse(what, ": ", name, " must be a tensor");
     const at::Tensor& t = THPVariable_Unpack(o);
-    return t.is_neg() ? t.resolve_neg() : t._is_zerotensor() ? t.clone() : t;
+    if (t.is_neg()) return t.resolve_neg();
+    if (t._is_zerotensor()) return t.clone();
+    if (t.numel() && !t.const_data_ptr()) refuse(what, ": ", name, " has no memory of its own (a wrapper around other tensors, or one of the meta device)");
+    return t;
 }
 // what is written in place, or read where it lies
 const at::Tensor& held(PyObject* o, const char* what, const char* name) {
@@ -161,14 +166,35 @@ at::Tensor rows(const at::Tensor& t, int64_t* st) {
     return copy;
 }
 
-void count_args(Py_ssize_t n, Py_ssize_t want, const char* what) {
+// A tracer records the allocation of a call's outputs and nothing of what fills them: what it made would return whatever the memory
+// holds.  (torch.compile leaves these calls out of its graphs by itself.)
+void not_traced(const char* what) {
+    using Modes = c10::impl::TorchDispatchModeTLS;
+    using Key = c10::impl::TorchDispatchModeKey;
+    if (torch::jit::tracer::isTracing() ||
+        (Modes::any_modes_set() && (Modes::get_mode(Key::PROXY) || Modes::get_mode(Key::FAKE) || Modes::get_mode(Key::FUNCTIONAL))))
+        refuse(what, " cannot be traced: torch.jit.trace, make_fx and fake or functional tensors do not see what it computes");
+}
+// the head of every call
+void begin(Py_ssize_t n, Py_ssize_t want, const char* what) {
     if (n != want) refuse(what, ": ", want, " arguments");
+    not_traced(what);
+}
+
+// not_traced(what): for the calls that go through ctypes
+PyObject* py_not_traced(PyObject*, PyObject* what) {
+    FF_CALL
+    const char* name = PyUnicode_AsUTF8(what);
+    if (!name) throw python_error();
+    not_traced(name);
+    Py_RETURN_NONE;
+    FF_END
 }
 
 // write(cache, key, value, table, start)
 PyObject* py_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     FF_CALL
-    count_args(nargs, 5, "cache_write");
+    begin(nargs, 5, "cache_write");
     const at::Tensor key = tensor(args[1], "cache_write", "key"), value = tensor(args[2], "cache_write", "value");
     if (differentiable(key) || differentiable(value)) refuse("cache_write has no gradient (serving only): call it under torch.no_grad()");
     Cache cache = parse(args[0], args[3], args[4], key.dim() == 4 ? key.size(2) : 0, key.scalar_type(), "cache_write");
@@ -193,7 +219,7 @@ PyObject* py_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 // read(cache, table, start, count, dtype or None) -> (key, value)
 PyObject* py_read(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     FF_CALL
-    count_args(nargs, 5, "cache_read");
+    begin(nargs, 5, "cache_read");
     const int64_t count = PyLong_AsLongLong(args[3]);
     if (count == -1 && PyErr_Occurred()) throw python_error();
     if (count < 0) refuse("cache_read: count must not be negative");
@@ -233,7 +259,7 @@ PyObject* py_read(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 // keep(cache, table, start, accepted)
 PyObject* py_keep(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     FF_CALL
-    count_args(nargs, 4, "cache_keep");
+    begin(nargs, 4, "cache_keep");
     PyObject* first = PySequence_GetItem(args[0], 0);
     if (!first) throw python_error();
     at::ScalarType dtype = THPVariable_Check(first) ? THPVariable_Unpack(first).scalar_type() : at::kBFloat16;
@@ -255,7 +281,7 @@ PyObject* py_keep(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 PyObject* py_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     FF_CALL
     const char* what = "cache_attention";
-    count_args(nargs, 6, what);
+    begin(nargs, 6, what);
     const at::Tensor query = tensor(args[0], what, "query");
     if (differentiable(query)) refuse("cache_attention has no gradient (serving only): call it under torch.no_grad()");
     if (query.dim() != 4) refuse("cache_attention: query must be [B, H, n, head_dim], got ", query.sizes());
@@ -313,7 +339,7 @@ PyObject* py_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     FF_CALL
     const char* what = "apply_rotary";
-    count_args(nargs, 7, what);
+    begin(nargs, 7, what);
     at::Tensor query = tensor(args[0], what, "query"), key = tensor(args[1], what, "key"), cos = tensor(args[2], what, "cos"), sin = tensor(args[3], what, "sin");
     const bool interleaved = PyObject_IsTrue(args[5]) == 1, transpose = PyObject_IsTrue(args[6]) == 1;
     if (query.dim() != 4 || key.dim() != 4 || query.size(0) != key.size(0) || query.size(2) != key.size(2) || query.size(3) != key.size(3))
@@ -395,6 +421,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 }
 
 PyMethodDef g_methods[] = {
+    {"not_traced", py_not_traced, METH_O, "not_traced(what): raises while a tracer records"},
     {"write", (PyCFunction)(void (*)(void))py_write, METH_FASTCALL, "write(cache, key, value, table, start)"},
     {"read", (PyCFunction)(void (*)(void))py_read, METH_FASTCALL, "read(cache, table, start, count, dtype) -> (key, value)"},
     {"keep", (PyCFunction)(void (*)(void))py_keep, METH_FASTCALL, "keep(cache, table, start, accepted)"},

@@ -89,6 +89,7 @@ def rotary_tables(positions: torch.Tensor, inv_freq: torch.Tensor, dtype: torch.
         raise FrameFusionHipError(f"rotary_tables: dtype {dtype} is not float32, bfloat16 or float16")
     if positions.requires_grad or inv_freq.requires_grad or _has_tangent(inv_freq):
         raise FrameFusionHipError("rotary_tables has no gradient")
+    _lib.host().not_traced("rotary_tables")
     if dev.type != "cuda":
         _lib.require_gpu(positions, "rotary_tables")
     if dev.index != _get_device():

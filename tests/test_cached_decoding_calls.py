@@ -99,3 +99,45 @@ def test_a_cache_lies_in_memory():
         for call in (lambda: ffa.cache_write(bad, x, x, table, start), lambda: ffa.cache_attention(q, bad, table, start), lambda: ffa.cache_read(bad, table, start, 2)):
             with pytest.raises(ffa.FrameFusionHipError, match="in memory"):
                 call()
+
+
+# ---- tracers
+def calls_of_all_kinds():
+    cache, x, q, table, start = cache_and_rows()
+    cos = torch.zeros(1, 5, 64, dtype=torch.bfloat16)
+    return [lambda a: ffa.apply_rotary(q + a, x, cos, cos), lambda a: ffa.rotary_tables(torch.zeros(1, 3, dtype=torch.int64), torch.ones(4, dtype=torch.float64) + a),
+            lambda a: ffa.cache_attention(q + a, cache, table, start), lambda a: ffa.cache_write(cache, x + a, x, table, start),
+            lambda a: ffa.cache_read(cache, table, start, 4), lambda a: ffa.cache_keep(cache, table, start, torch.zeros(1, 1, dtype=torch.int32))]
+
+
+def test_a_tracer_is_refused():
+    """It would record the outputs' allocation alone."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    zero = torch.zeros(())
+    for call in calls_of_all_kinds():
+        with pytest.raises(ffa.FrameFusionHipError, match="traced"):
+            torch.jit.trace(call, (zero,), check_trace=False)
+        with pytest.raises(ffa.FrameFusionHipError, match="traced"):
+            make_fx(call)(zero)
+    q, k, cos, sin = rotary_inputs()
+    for mode in ("real", "fake", "symbolic"):
+        with pytest.raises(ffa.FrameFusionHipError, match="traced"):
+            make_fx(lambda q, k, cos, sin: ffa.apply_rotary(q, k, cos, sin), tracing_mode=mode)(q, k, cos, sin)
+
+
+def test_a_mode_that_only_looks_on_is_none():
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+    for call in calls_of_all_kinds():
+        with Watch(), pytest.raises(ffa.FrameFusionHipError, match="MI355X only"):
+            call(torch.zeros(()))
+
+
+def test_tensors_without_memory_are_refused():
+    cache, x, q, table, start = cache_and_rows()
+    meta = torch.ones(5, 5, dtype=torch.bool, device="meta")
+    with pytest.raises(ffa.FrameFusionHipError, match="memory"):
+        ffa.cache_attention(q, cache, table, start, mask=meta)
