@@ -209,12 +209,12 @@ _lib = None
 
 
 def hashed_sources():
-    """The files csrc/Makefile hashes into the library (its HASHED list: SRCS + HDRS + the public header + itself), read
+    """The files csrc/Makefile hashes into the binaries (its HASHED list: SRCS + HDRS + HOSTSRC + the public header + itself), read
     from the Makefile so that the two lists cannot drift apart."""
     import re
     text = open(os.path.join(CSRC, "Makefile")).read().replace("\\\n", " ")
     names = []
-    for var in ("SRCS", "HDRS"):
+    for var in ("SRCS", "HDRS", "HOSTSRC"):
         m = re.search(rf"^{var}\s*=\s*(.*)$", text, re.M)
         if m is None:
             raise FrameFusionHipError(f"csrc/Makefile has no {var} line")
@@ -266,6 +266,28 @@ def file_stamp(path: str = None):
     return blob[at + 10:at + 26].decode("ascii", "replace") if at >= 0 else "(a library from before the stamp)"
 
 
+def _refuse_stale(path: str) -> None:
+    """A stale binary (sources edited since it was built, a build that broke off between the two, or a copy whose timestamps hide that
+    from make) is rebuilt, never run: the stamp is read from the file BEFORE anything is loaded.  Rebuilding needs make + hipcc: a
+    deployment that ships sources next to a binary built from OTHER sources, without a compiler, gets an error that says so
+    (FF_AUTO_BUILD=0 turns the implicit build off altogether)."""
+    want = source_hash()
+    if want is None or file_stamp(path) == want:
+        return
+    import shutil
+    if os.environ.get("FF_AUTO_BUILD", "1") == "0" or not (shutil.which("make") and shutil.which(os.environ.get("HIPCC", "hipcc"))):
+        raise FrameFusionHipError(
+            f"{path} was built from other sources (its stamp {file_stamp(path)}, the sources' {want}) and this process may "
+            f"not or cannot rebuild it (FF_AUTO_BUILD=0, or make / hipcc not on PATH): run `make -C {CSRC}` where a ROCm "
+            f"toolchain is installed, or ship the binaries without the csrc/ directory")
+    build()
+    if file_stamp(path) != want:
+        build(force=True)
+    if file_stamp(path) != want:
+        raise FrameFusionHipError(f"{path} was built from other sources (its stamp {file_stamp(path)}, the sources' "
+                                  f"{want}) and rebuilding did not change that")
+
+
 def load():
     global _lib
     if _lib is not None:
@@ -278,24 +300,7 @@ def load():
             raise FrameFusionHipError(
                 f"{LIB_PATH} is missing and could not be built ({e}): run `python -c 'import __graft_entry__ as g; "
                 f"g.build()'` (or `make -C {CSRC}`). framefusion_amd has no CPU/eager fallback.") from e
-    # a stale binary (sources edited since it was built, or a copy whose timestamps hide that from make) is rebuilt,
-    # never run: the stamp is read from the file BEFORE anything is loaded.  Rebuilding needs make + hipcc: a deployment
-    # that ships sources next to a binary built from OTHER sources, without a compiler, gets an error that says so
-    # (FF_AUTO_BUILD=0 turns the implicit build off altogether).
-    want = source_hash()
-    if want is not None and file_stamp() != want:
-        import shutil
-        if os.environ.get("FF_AUTO_BUILD", "1") == "0" or not (shutil.which("make") and shutil.which(os.environ.get("HIPCC", "hipcc"))):
-            raise FrameFusionHipError(
-                f"{LIB_PATH} was built from other sources (its stamp {file_stamp()}, the sources' {want}) and this process may "
-                f"not or cannot rebuild it (FF_AUTO_BUILD=0, or make / hipcc not on PATH): run `make -C {CSRC}` where a ROCm "
-                f"toolchain is installed, or ship the library without the csrc/ directory")
-        build()
-        if file_stamp() != want:
-            build(force=True)
-        if file_stamp() != want:
-            raise FrameFusionHipError(f"{LIB_PATH} was built from other sources (its stamp {file_stamp()}, the sources' "
-                                      f"{want}) and rebuilding did not change that")
+    _refuse_stale(LIB_PATH)
     try:
         lib = C.CDLL(LIB_PATH)
     except OSError as e:  # pragma: no cover
@@ -322,9 +327,10 @@ def host():
     """framefusion_amd._host (csrc/ff_host.cpp, built with the library): the cached-decoding calls in one crossing each."""
     global _host
     if _host is None:
-        load()                               # (rebuilds both when the sources have changed)
+        load()
         if not os.path.exists(HOST_PATH):
             build()
+        _refuse_stale(HOST_PATH)
         try:
             import importlib
             _host = importlib.import_module("framefusion_amd._host")

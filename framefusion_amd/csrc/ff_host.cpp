@@ -20,7 +20,11 @@
 #include <sstream>
 #include <string>
 
+#include "ff_source_hash.h"
 #include "framefusion_hip.h"
+
+// what this module was built from, readable from the file
+extern "C" __attribute__((visibility("default"), used)) const char ff_host_stamp[] = "FFSRCHASH:" FF_SOURCE_HASH;
 
 namespace {
 
@@ -433,6 +437,14 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_host", "checks, outputs and lau
 }  // namespace
 
 PyMODINIT_FUNC PyInit__host(void) {
+    // the structures below are passed to the library as they are: both must come from the same sources
+    const size_t mine[4] = {sizeof(ff_rotary_t), sizeof(ff_cache_t), sizeof(ff_cache_rows_t), sizeof(ff_cache_attention_t)};
+    bool same = std::string(ff_source_hash()) == ff_host_stamp + 10;
+    for (int i = 0; i < 4; ++i) same = same && ff_abi_sizeof(6 + i) == mine[i];
+    if (!same) {
+        PyErr_Format(PyExc_ImportError, "_host.so was built from other sources (%s) than the library beside it (%s)", ff_host_stamp + 10, ff_source_hash());
+        return nullptr;
+    }
     PyObject* lib = PyImport_ImportModule("framefusion_amd._lib");
     if (!lib) return nullptr;
     g_error = PyObject_GetAttrString(lib, "FrameFusionHipError");
