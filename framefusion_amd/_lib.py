@@ -236,12 +236,13 @@ def source_hash() -> str:
     return h.hexdigest()[:16]
 
 
-def build(verbose: bool = False, force: bool = False) -> str:
-    """Compile the HIP sources in csrc/ for gfx950 (hipcc cross-compiles without a GPU).  `force`: recompile every
-    file (`make -B`) - what __graft_entry__.build() does, so that "it built" means "these sources compile"."""
+def build(verbose: bool = False, force: bool = False, target: str = "all") -> str:
+    """Compile the HIP sources in csrc/ for gfx950 (hipcc cross-compiles without a GPU) and the host module beside them.  `force`: recompile every
+    file (`make -B`) - what __graft_entry__.build() does, so that "it built" means "these sources compile".  `target` "lib": the
+    library alone, which needs neither g++ nor the headers of torch and Python."""
     if not os.path.isdir(CSRC):
         raise FrameFusionHipError(f"{CSRC} not found")
-    cmd = ["make", "-C", CSRC, "-j", str(min(8, os.cpu_count() or 1))] + (["-B"] if force else [])
+    cmd = ["make", "-C", CSRC, target, "-j", str(min(8, os.cpu_count() or 1))] + (["-B"] if force else [])
     # one build at a time: several ranks of one job may find the same stale binary at the same moment
     import fcntl
     with open(os.path.join(CSRC, ".build.lock"), "w") as lock:
@@ -251,7 +252,7 @@ def build(verbose: bool = False, force: bool = False) -> str:
         print(res.stdout[-4000:])
         print(res.stderr[-4000:])
     if res.returncode:
-        raise FrameFusionHipError("building libframefusion_hip.so failed (see output above)")
+        raise FrameFusionHipError(f"building {'libframefusion_hip.so' if target == 'lib' else 'libframefusion_hip.so and _host.so'} failed (see output above)")
     return LIB_PATH
 
 
@@ -266,7 +267,7 @@ def file_stamp(path: str = None):
     return blob[at + 10:at + 26].decode("ascii", "replace") if at >= 0 else "(a library from before the stamp)"
 
 
-def _refuse_stale(path: str) -> None:
+def _refuse_stale(path: str, target: str) -> None:
     """A stale binary (sources edited since it was built, a build that broke off between the two, or a copy whose timestamps hide that
     from make) is rebuilt, never run: the stamp is read from the file BEFORE anything is loaded.  Rebuilding needs make + hipcc: a
     deployment that ships sources next to a binary built from OTHER sources, without a compiler, gets an error that says so
@@ -278,11 +279,11 @@ def _refuse_stale(path: str) -> None:
     if os.environ.get("FF_AUTO_BUILD", "1") == "0" or not (shutil.which("make") and shutil.which(os.environ.get("HIPCC", "hipcc"))):
         raise FrameFusionHipError(
             f"{path} was built from other sources (its stamp {file_stamp(path)}, the sources' {want}) and this process may "
-            f"not or cannot rebuild it (FF_AUTO_BUILD=0, or make / hipcc not on PATH): run `make -C {CSRC}` where a ROCm "
+            f"not or cannot rebuild it (FF_AUTO_BUILD=0, or make / hipcc not on PATH): run `make -C {CSRC} all` where a ROCm "
             f"toolchain is installed, or ship the binaries without the csrc/ directory")
-    build()
+    build(target=target)
     if file_stamp(path) != want:
-        build(force=True)
+        build(force=True, target=target)
     if file_stamp(path) != want:
         raise FrameFusionHipError(f"{path} was built from other sources (its stamp {file_stamp(path)}, the sources' "
                                   f"{want}) and rebuilding did not change that")
@@ -295,12 +296,12 @@ def load():
     if not os.path.exists(LIB_PATH):
         # not built yet (fresh checkout): compile the HIP sources once, in-tree; there is no other path
         try:
-            build()
+            build(target="lib")
         except Exception as e:
             raise FrameFusionHipError(
                 f"{LIB_PATH} is missing and could not be built ({e}): run `python -c 'import __graft_entry__ as g; "
-                f"g.build()'` (or `make -C {CSRC}`). framefusion_amd has no CPU/eager fallback.") from e
-    _refuse_stale(LIB_PATH)
+                f"g.build()'` (or `make -C {CSRC} all`). framefusion_amd has no CPU/eager fallback.") from e
+    _refuse_stale(LIB_PATH, "lib")
     try:
         lib = C.CDLL(LIB_PATH)
     except OSError as e:  # pragma: no cover
@@ -330,12 +331,12 @@ def host():
         load()
         if not os.path.exists(HOST_PATH):
             build()
-        _refuse_stale(HOST_PATH)
+        _refuse_stale(HOST_PATH, "all")
         try:
             import importlib
             _host = importlib.import_module("framefusion_amd._host")
         except ImportError as e:
-            raise FrameFusionHipError(f"cannot load {HOST_PATH}: {e} (built with another torch? run `make -C {CSRC}`); there is no other path") from e
+            raise FrameFusionHipError(f"cannot load {HOST_PATH}: {e} (built with another torch? run `make -C {CSRC} all`); there is no other path") from e
     return _host
 
 

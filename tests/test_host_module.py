@@ -48,3 +48,22 @@ def test_a_module_of_another_build_than_the_library_is_not_loaded(tree):
     shutil.rmtree(pkg / "csrc")
     out = run()
     assert "refused:" in out.stdout and "0123456789abcdef" in out.stdout and "than the library beside it" in out.stdout, out
+
+
+def test_the_library_alone_needs_no_torch_to_build():
+    """make without a target is what a host of the C ABI runs; the package's own build makes both."""
+    def commands(*target):
+        return subprocess.run(["make", "-n", "-B", "-C", _lib.CSRC, *target], capture_output=True, text=True, check=True).stdout
+    assert "-ltorch" not in commands() and "-o ../libframefusion_hip" in commands()
+    assert "-ltorch" in commands("all")
+
+
+def test_the_library_is_built_without_the_module(monkeypatch, tmp_path):
+    """A process that only reduces prefills asks for the library alone, also where it has to build it."""
+    asked = []
+    monkeypatch.setattr(_lib, "build", lambda verbose=False, force=False, target="all": asked.append(target))
+    monkeypatch.setattr(_lib, "_lib", None)
+    monkeypatch.setattr(_lib, "LIB_PATH", str(tmp_path / "nope.so"))
+    with pytest.raises(_lib.FrameFusionHipError):
+        _lib.load()
+    assert asked and set(asked) == {"lib"}
