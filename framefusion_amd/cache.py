@@ -88,6 +88,9 @@ class ReducedCache:
     runs ``cache_attention`` over them.  A call with ``tree_mask`` (bool [n, n]) attends as a tree of drafted tokens and leaves them
     pending until ``keep(accepted)``.
 
+    ``seen`` counts the tokens that the model was given, before any reduction: where the next one's position follows on (every layer
+    holds fewer, even the first, whose call comes behind a reduction).  ``lengths`` is what each layer holds.
+
     ``max_tokens`` bounds the length of every layer; ``pages`` the pool (default: enough for ``max_tokens`` everywhere - a reduced
     prefill needs far fewer).  One instance serves one stream of calls, like the reference's module; after a step that raised, ``reset``."""
 
@@ -98,6 +101,7 @@ class ReducedCache:
         width = -(-max_tokens // page_size) if page_size > 0 else 0
         self.tensors = new_cache(layers * width if pages is None else pages, page_size, kv_heads, head_dim, dtype, store, device)
         self.dtype, self.page_size, self.max_tokens = dtype, page_size, max_tokens
+        self.seen = 0                               # tokens given to the model, without pending ones
         self.lengths = [0] * layers                 # tokens held, without pending ones
         self.pending = [0] * layers                 # tokens written behind them by the current step
         self._pages = [[] for _ in range(layers)]
@@ -108,7 +112,8 @@ class ReducedCache:
         self._rows = [(self._table[i:i + 1], self._start[i:i + 1]) for i in range(layers)]
 
     def get_seq_length(self, layer_idx: int = 0) -> int:
-        return self.lengths[layer_idx]
+        """``seen``, for every layer: callers count positions on from it."""
+        return self.seen
 
     def __len__(self) -> int:
         return len(self.lengths)
@@ -146,8 +151,9 @@ class ReducedCache:
             raise FrameFusionHipError(f"ReducedCache: {self.pending[layer]} tokens are pending in layer {layer}, query is {tuple(query.shape)}")
         return cache_attention(query, self.tensors, *self._rows[layer], mask=mask, scale=scale)
 
-    def _count(self, added):
-        """The pending tokens of every layer become `added` held ones."""
+    def _count(self, added, tokens):
+        """The pending tokens of every layer become `added` held ones, `tokens` of the model's."""
+        self.seen += tokens
         self.lengths = [n + a for n, a in zip(self.lengths, added)]
         self.pending = [0] * len(added)
         if min(added) == max(added):
@@ -156,9 +162,13 @@ class ReducedCache:
         else:
             self._start.copy_(torch.tensor(self.lengths, dtype=torch.int32))
 
-    def advance(self) -> None:
-        """Every pending token counts from now on."""
-        self._count(self.pending)
+    def advance(self, tokens: Optional[int] = None) -> None:
+        """Every pending token counts from now on.  ``tokens``: how many the model was given, where layers were written fewer (a reduced
+        prefill); by default as many as the fullest layer was written."""
+        most = max(self.pending)
+        if tokens is not None and tokens < most:
+            raise FrameFusionHipError(f"ReducedCache: {most} tokens are pending in a layer, the model cannot have been given {tokens}")
+        self._count(self.pending, most if tokens is None else tokens)
 
     def keep(self, accepted) -> None:
         """Of the pending drafted tokens the ``accepted`` ones (increasing indices, the same in every layer) stay, in one launch for all
@@ -171,7 +181,7 @@ class ReducedCache:
         if accepted and accepted != list(range(len(accepted))):
             lists = torch.tensor(accepted, dtype=torch.int32, device=self._table.device).expand(len(self.lengths), -1).contiguous()
             cache_keep(self.tensors, self._table, self._start, lists)
-        self._count([len(accepted)] * len(self.lengths))
+        self._count([len(accepted)] * len(self.lengths), len(accepted))
 
     def dense(self, layer: int) -> Tuple[torch.Tensor, torch.Tensor]:
         """The layer's keys and values [1, kv_heads, length, head_dim], read back."""
@@ -184,4 +194,4 @@ class ReducedCache:
             have.clear()
         self._table.fill_(-1)
         self._start.zero_()
-        self.lengths, self.pending = [0] * len(self.lengths), [0] * len(self.lengths)
+        self.seen, self.lengths, self.pending = 0, [0] * len(self.lengths), [0] * len(self.lengths)

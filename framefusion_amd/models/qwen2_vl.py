@@ -17,13 +17,11 @@ With a ``ReducedCache`` as ``past_key_values`` the layers rotate with ``apply_ro
 """
 from __future__ import annotations
 
-import torch
-
 from ..cache import ReducedCache
 from ..interface import Family, register_family
 from ..main import call_b_with_residual
 from ..utils import last_query_importance
-from .cached import cached_attention, continues, finish_step, position_tables, prefill_mask, rotate
+from .cached import cached_attention, continues, default_positions, finish_step, position_tables, prefill_mask, rotate
 
 NUM_IMPORTANCE_QUERIES = 4           # modeling_qwen2_vl.py:296
 
@@ -99,8 +97,7 @@ def qwen2vl_text_model_forward(self, input_ids=None, attention_mask=None, positi
     if use_cache and past_key_values is None:
         past_key_values = DynamicCache(config=self.config)
     if position_ids is None:
-        seen = past_key_values.get_seq_length() if past_key_values is not None else 0
-        position_ids = (torch.arange(inputs_embeds.shape[1], device=inputs_embeds.device) + seen)
+        position_ids = default_positions(past_key_values, inputs_embeds.shape[1], inputs_embeds.device, kwargs.get("tree_mask"))
         position_ids = position_ids.view(1, 1, -1).expand(3, inputs_embeds.shape[0], -1)
     elif position_ids.ndim == 2:
         position_ids = position_ids[None, ...].expand(3, position_ids.shape[0], -1)
@@ -123,7 +120,7 @@ def qwen2vl_text_model_forward(self, input_ids=None, attention_mask=None, positi
             position_ids=None, past_key_values=past_key_values, use_cache=use_cache, **kwargs)
         lengths.append(hidden_states.shape[1])
     self.framefusion_lengths = lengths
-    finish_step(past_key_values, kwargs.get("tree_mask"))
+    finish_step(past_key_values, kwargs.get("tree_mask"), inputs_embeds.shape[1])
     hidden_states = self.norm(hidden_states)
     return BaseModelOutputWithPast(last_hidden_state=hidden_states, past_key_values=past_key_values)
 
