@@ -118,6 +118,12 @@ class ReducedCache:
     def __len__(self) -> int:
         return len(self.lengths)
 
+    @property
+    def is_compileable(self):
+        """What transformers' ``generate`` asks first."""
+        raise NotImplementedError("model.generate does not take a ReducedCache (it passes an attention_mask and drives the cache by one length for all layers): "
+                                  "call the model once for the prompt and once for each token, or leave past_key_values to generate")
+
     def _room(self, layer, count):
         """Pages for `count` tokens of a layer."""
         if count > self.max_tokens:
