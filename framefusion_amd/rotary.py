@@ -20,56 +20,90 @@ _get_device = torch._C._cuda_getDevice
 _CODE = _lib.DTYPE_CODE
 
 
-def rotary_frequencies(dim: int, base: float = 10000.0, scaling: Optional[dict] = None) -> Tuple[torch.Tensor, float]:
-    """(float64 frequencies [dim / 2] on the CPU, factor on cosine and sine) for ``rotary_tables``.  ``scaling`` stretches the
-    positions for contexts longer than the trained one, in transformers' ``rope_parameters`` spelling:
+# what a scaling dictionary may hold beside rope_type (or type) and rope_theta: (needed, optional)
+_SCALING = {"default": ((), ()), "linear": (("factor",), ()), "ntk": (("factor",), ()),
+            "yarn": (("factor", "original_max_position_embeddings"), ("beta_fast", "beta_slow", "attention_factor", "mscale", "mscale_all_dim", "truncate")),
+            "llama3": (("factor", "low_freq_factor", "high_freq_factor", "original_max_position_embeddings"), ())}
+
+
+def rotary_frequencies(dim: int, base: Optional[float] = None, scaling: Optional[dict] = None) -> Tuple[torch.Tensor, float]:
+    """(float64 frequencies [dim / 2] on the CPU, factor on cosine and sine) for ``rotary_tables``.  ``dim`` is the number of rotated
+    channels; ``base`` is 10000, or what ``scaling`` says under "rope_theta".  ``scaling`` stretches the positions for contexts longer than
+    the trained one, in transformers' ``rope_parameters`` spelling:
 
     * ``{"rope_type": "linear", "factor": s}``: every frequency divided by s;
     * ``{"rope_type": "ntk", "factor": s}``: the base raised to base * s^(dim / (dim - 2)), which divides the slowest pair by s and
       leaves the fastest alone;
-    * ``{"rope_type": "yarn", "factor": s, "original_max_position_embeddings": n[, "beta_fast": 32, "beta_slow": 1,
-      "attention_factor": 0.1 ln s + 1]}``: pairs that turn more than beta_fast times over n positions are left alone, those below
-      beta_slow turns divided by s, the ones between blended by their index;
+    * ``{"rope_type": "yarn", "factor": s, "original_max_position_embeddings": n[, "beta_fast": 32, "beta_slow": 1, "truncate": True,
+      "attention_factor", or "mscale" with "mscale_all_dim"]}``: pairs that turn more than beta_fast times over n positions are left
+      alone, those below beta_slow turns divided by s, the ones between blended by their index (its ends rounded to whole pairs unless
+      "truncate" is false).  The factor is "attention_factor", else g(mscale) / g(mscale_all_dim) where both are there, else g(1), with
+      g(m) = 0.1 m ln s + 1 (1 for s <= 1);
     * ``{"rope_type": "llama3", "factor": s, "low_freq_factor": a, "high_freq_factor": b, "original_max_position_embeddings": n}``:
       pairs with a wavelength above n / a divided by s, below n / b left alone, blended by n / wavelength between.
-    """
+
+    An entry of None counts as left out, "mrope_section" (which is ``apply_rotary``'s) is passed over, any other entry is refused."""
     if dim < 2 or dim % 2:
         raise FrameFusionHipError(f"rotary dimension must be even and positive, got {dim}")
+    scaling = {k: v for k, v in (scaling or {}).items() if v is not None and k != "mrope_section"}
+    theta = scaling.pop("rope_theta", None)
+    if base is not None and theta is not None and float(base) != float(theta):
+        raise FrameFusionHipError(f"rotary base {base} and rope_theta {theta} differ")
+    base = float(base if base is not None else theta if theta is not None else 10000.0)
+    if not base > 0:
+        raise FrameFusionHipError(f"rotary base must be positive, got {base}")
+    if scaling.pop("partial_rotary_factor", 1) != 1:
+        raise FrameFusionHipError("rotary dimension is the number of rotated channels: pass head_dim * partial_rotary_factor and leave the entry out")
+    older = scaling.pop("type", "default")
+    kind = scaling.pop("rope_type", older)
+    if kind not in _SCALING:
+        raise FrameFusionHipError(f"rotary scaling {kind!r} is not one of {', '.join(_SCALING)}")
+    needed, optional = _SCALING[kind]
+    missing, unknown = [k for k in needed if k not in scaling], [k for k in scaling if k not in needed + optional]
+    if missing or unknown:
+        raise FrameFusionHipError(f"rotary scaling {kind!r}" + (f" needs {', '.join(missing)}" if missing else "") + (f" does not know {', '.join(unknown)}" if unknown else ""))
     pair = torch.arange(0, dim, 2, dtype=torch.float64)
-    inv = float(base) ** (-pair / dim)
-    if scaling is None:
-        return inv, 1.0
-    kind = scaling.get("rope_type", scaling.get("type", "default"))
+    inv = base ** (-pair / dim)
     if kind == "default":
         return inv, 1.0
     s = float(scaling["factor"])
-    if s <= 0:
+    if not s > 0:
         raise FrameFusionHipError(f"rotary scaling factor must be positive, got {s}")
     if kind == "linear":
         return inv / s, 1.0
     if kind == "ntk":
         if dim == 2:
             raise FrameFusionHipError("ntk scaling needs more than one pair")
-        return (float(base) * s ** (dim / (dim - 2))) ** (-pair / dim), 1.0
+        return (base * s ** (dim / (dim - 2))) ** (-pair / dim), 1.0
+    n = float(scaling["original_max_position_embeddings"])
+    if not n > 0:
+        raise FrameFusionHipError(f"original_max_position_embeddings must be positive, got {n}")
     if kind == "yarn":
-        n = float(scaling["original_max_position_embeddings"])
         fast, slow = float(scaling.get("beta_fast") or 32), float(scaling.get("beta_slow") or 1)
+        if not (base > 1 and fast > 0 and slow > 0):
+            raise FrameFusionHipError(f"yarn scaling needs a base above 1 and positive beta_fast and beta_slow, got {base}, {fast}, {slow}")
 
         def index_of(turns):                      # the (fractional) pair index that turns `turns` times over n positions
-            return dim * math.log(n / (turns * 2 * math.pi)) / (2 * math.log(float(base)))
-        low, high = max(math.floor(index_of(fast)), 0), min(math.ceil(index_of(slow)), dim - 1)
+            return dim * math.log(n / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+        def gain(m):
+            return 0.1 * m * math.log(s) + 1.0 if s > 1 else 1.0
+        low, high = index_of(fast), index_of(slow)
+        if scaling.get("truncate", True):
+            low, high = math.floor(low), math.ceil(high)
+        low, high = max(low, 0), min(high, dim - 1)
         ramp = ((torch.arange(dim // 2, dtype=torch.float64) - low) / max(high - low, 1e-3)).clamp(0, 1)
         factor = scaling.get("attention_factor")
         if factor is None:
-            factor = 0.1 * math.log(s) + 1.0 if s > 1 else 1.0
+            one, other = scaling.get("mscale"), scaling.get("mscale_all_dim")
+            factor = gain(float(one)) / gain(float(other)) if one and other else gain(1.0)
         return inv / s * ramp + inv * (1 - ramp), float(factor)
-    if kind == "llama3":
-        n = float(scaling["original_max_position_embeddings"])
-        a, b = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
-        turns = n * inv / (2 * math.pi)                                 # n / wavelength
-        keep = ((turns - a) / (b - a)).clamp(0, 1)
-        return inv / s * (1 - keep) + inv * keep, 1.0
-    raise FrameFusionHipError(f"rotary scaling {kind!r} is not one of default, linear, ntk, yarn, llama3")
+    a, b = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+    if not b > a:
+        raise FrameFusionHipError(f"llama3 scaling needs high_freq_factor above low_freq_factor, got {b} and {a}")
+    turns = n * inv / (2 * math.pi)                                     # n / wavelength
+    keep = ((turns - a) / (b - a)).clamp(0, 1)
+    return inv / s * (1 - keep) + inv * keep, 1.0
 
 
 def _has_tangent(*tensors) -> bool:
