@@ -223,6 +223,8 @@ template <int DT, int STORE, int DH> __device__ inline bool take_out_odd(Raw<DT,
 // Registers: keys and values of two steps (one in use, one on its way), Q and the outputs.  Where they pass 256 the kernel runs one wave a
 // SIMD with 512 (one token of 28 / 4 fp32 heads of 128 over 8 x 20 000 keys: 257 us spilling, 148 us so); fp32 rows of 256 channels
 // pass 512 too and are loaded when they are needed (587 us spilling, 269 us so): 64 KB a wave in flight are enough for the memory.
+// bf16 and fp16 rows of 128 channels in two tiles are 3 and 5 registers too many for 256, which go to memory and back: 35 rows a kv head over
+// 4 x 13 474 keys take 49 us so and 63 us with one wave a SIMD.
 constexpr int waves_a_simd(int dt, int store, int dh, int nt) {
     const int bytes = store == kStoreSame && dt == FF_F32 ? 4 : 2;
     return dh * nt * bytes > 512 || dh == 256 || (bytes == 4 && dh == 128) ? 1 : 2;
@@ -232,6 +234,9 @@ __global__ __launch_bounds__(64 * kAttWaves, waves_a_simd(DT, STORE, DH, NT)) vo
     using G = Geo<DT, STORE, DH>;
     constexpr int kSteps = DH / 32, kTiles = DH / 16, kPad = 4;
     constexpr bool kAhead = !(DT == FF_F32 && STORE == kStoreSame && DH == 256);
+    // Two tiles of 256 channels pass 512 registers by far.  What the compiler then spills it splits between accumulation registers and
+    // memory, and in the 8-bit form it brought the first fragment of the first tile's Q back without its third word: wrong scores.
+    static_assert(NT == 1 || DH <= (DT == FF_F32 ? 64 : 128), "two tiles of rows must leave the registers room");
     __shared__ float s_o[kAttWaves][16][DH + kPad];
     __shared__ float s_m[kAttWaves][16], s_l[kAttWaves][16];
     const ff_cache_t& c = a.cache;
