@@ -156,8 +156,7 @@ class _Rotary(torch.autograd.Function):
             raise FrameFusionHipError("apply_rotary: a differentiable call cannot be captured into a graph (use transpose=True on the gradients)")
         cos, sin = ctx.saved_tensors
         sections, interleaved, transpose = ctx.how
-        turn = _Rotary.apply if torch.is_grad_enabled() else _lib.host().rotary           # (differentiated again, or the end of the line)
-        dq, dk = turn(dq, dk, cos, sin, sections, interleaved, not transpose)
+        dq, dk = apply_rotary(dq, dk, cos, sin, sections, interleaved, not transpose)          # (differentiated again where that is asked for)
         return dq, dk, None, None, None, None, None
 
     @staticmethod

@@ -61,6 +61,9 @@ def test_the_rotation_carries_tangents(formula):
         y, _ = ffa.apply_rotary(x, k, cos, sin)
         grad, = torch.autograd.grad(y, x, forward_ad.make_dual(g, dg), create_graph=True)
         assert torch.equal(forward_ad.unpack_dual(grad).tangent, ffa.apply_rotary(dg, k, cos, sin, transpose=True)[0])
+        y, _ = ffa.apply_rotary(x, k, cos, sin)
+        grad, = torch.autograd.grad(y, x, forward_ad.make_dual(g, dg))                # (the backward graph is not kept: its tangent is)
+        assert torch.equal(forward_ad.unpack_dual(grad).tangent, ffa.apply_rotary(dg, k, cos, sin, transpose=True)[0])
         with pytest.raises(ffa.FrameFusionHipError, match="constants"):
             ffa.apply_rotary(forward_ad.make_dual(q, dq), k, forward_ad.make_dual(cos, cos), sin)
 
