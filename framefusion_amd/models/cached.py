@@ -38,6 +38,8 @@ def position_tables(model, cache, hidden_states, position_ids, attention_mask, t
     rotary = model.rotary_emb
     if getattr(rotary, "rope_type", "default") in ("dynamic", "longrope"):      # (frequencies that follow the length)
         return list(rotary(hidden_states, position_ids))
+    if not position_ids.is_floating_point():
+        position_ids = position_ids.long()
     return list(rotary_tables(position_ids.contiguous(), rotary.inv_freq.double(), dtype=hidden_states.dtype, factor=rotary.attention_scaling))
 
 

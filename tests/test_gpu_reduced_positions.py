@@ -33,3 +33,17 @@ def test_default_positions(family):
             if tree is not None:
                 told.keep([0, 2, 4]), left.keep([0, 2, 4])
             at += n
+
+
+def test_positions_of_other_integer_types():
+    model, cfg = qwen2()
+    emb, pt = video_tokens(F_, P, D, p_change=0.5, sigma=0.3, sigma_hi=1.2, seed=11, pre=PRE, post=POST, dtype=torch.float32)
+    emb = emb.to(DEV)
+    caches = [ffa.ReducedCache(4, 2, 32, 512, dtype=torch.float32, page_size=16, device=DEV) for _ in range(2)]
+    x = torch.randn(1, 2, D, generator=torch.Generator(device=DEV).manual_seed(4), device=DEV)
+    with torch.no_grad():
+        for c in caches:
+            prefill(model, c, emb, pt)
+        got, want = (model.model(inputs_embeds=x, past_key_values=c, use_cache=True, position_ids=positions("qwen2", [310, 311]).to(t)).last_hidden_state
+                     for c, t in zip(caches, (torch.int32, torch.int64)))
+        assert torch.equal(got, want)
