@@ -11,7 +11,7 @@ as zeros and are not attended to.  `start` int32 [B] is the number of tokens a s
 negative entry marks a padding row of the batch.
 
 A stored value is code * 2^(scale byte - 127), one scale for 32 channels; scales are powers of two, so quantising rounds each
-channel once and reading back rounds nothing.  A block that holds a NaN or an infinity is stored as NaN.
+channel once and reading back in the type that was written rounds nothing.  A block that holds a NaN or an infinity is stored as NaN.
 """
 from __future__ import annotations
 
@@ -75,7 +75,10 @@ def cache_attention(query: torch.Tensor, cache, table: torch.Tensor, start: torc
     [n, n] or [B, n, n], a tree of drafted tokens: its ancestors and itself - is true; without a mask new token j <= i.  What a
     token does not see contributes nothing, whatever is stored there; one that sees nothing (and a padding row) gets zeros.
 
-    H is a multiple of the cache's heads, head_dim 32, 64, 128 or 256.  Returns [B, H, n, head_dim], laid out so that
+    Scores, statistics and sums are held in fp32; a weight is rounded to the inputs' type before it meets the value.  An infinity among the
+    values of earlier tokens comes out as one, or as NaN where its weight is below that type's smallest number.
+
+    H is a multiple of the cache's heads, head_dim 32, 64, 128 or 256, n * H at most 983 024.  Returns [B, H, n, head_dim], laid out so that
     ``out.transpose(1, 2)`` is contiguous."""
     return _lib.host().attention(query, cache, table, start, mask, scale)
 

@@ -221,8 +221,8 @@ template <int DT, int STORE, int DH> __device__ inline bool take_out_odd(Raw<DT,
 }
 
 // Registers: keys and values of two steps (one in use, one on its way), Q and the outputs.  Where they pass 256 the kernel runs one wave a
-// SIMD with 512 (one token of 28 / 4 fp32 heads of 128 over 8 x 20 000 keys: 257 us spilling, 148 us so); fp32 rows of 256 channels
-// pass 512 too and are loaded when they are needed (587 us spilling, 269 us so): 64 KB a wave in flight are enough for the memory.
+// SIMD with 512 (one token of 28 / 4 fp32 heads of 128 over 8 x 20 000 keys: 257 us spilling, 140 us so); fp32 rows of 256 channels
+// pass 512 too and are loaded when they are needed (587 us spilling, 267 us so): 64 KB a wave in flight are enough for the memory.
 // bf16 and fp16 rows of 128 channels in two tiles are 3 and 5 registers too many for 256, which go to memory and back: 35 rows a kv head over
 // 4 x 13 474 keys take 49 us so and 63 us with one wave a SIMD.
 constexpr int waves_a_simd(int dt, int store, int dh, int nt) {
@@ -604,8 +604,13 @@ static int attention_check(const ff_cache_attention_t* a) {
 
 // Which kernel serves R query rows, and how many waves share a block of keys there.  Up to 128 rows (and fp32, whose products are
 // slow anyway): 0, ff_attend.hip, whose waves hold 16 or 32 rows and read the cache again for the rows of the next workgroup; more:
-// ff_attend_rows.hip, tiles of 32 rows, a wave each.  4 sequences of 13 474, 28 / 4 heads of 128 in 8 bits: 84 rows 59 us here and 68
-// there, 126 rows 57 and 71, 252 rows 84 and 65.
+// ff_attend_rows.hip, tiles of 32 rows, a wave each.  A call over 4 sequences of 13 474, 28 / 4 heads of 128, here / there in us:
+//   rows       35         63         84         126        168        252
+//   bf16   49 / 38    55 / 41    69 / 38    57 / 40    90 / 50    84 / 53
+//   8 bits 39 / 39    46 / 42    53 / 39    53 / 41    67 / 51    78 / 54
+//   4 bits 34 / 39    39 / 42    45 / 40    46 / 42    60 / 50    70 / 53
+// Heads of 64 and 256 and a single sequence cross at the same place: at about 32 rows for a cache in T, 64 for codes.  From there to 128
+// the kernel there is ahead, by up to 1.8 (2.2 at 256 channels): the border was set before that kernel fed its products as it does now.
 static int row_waves(int dtype, int64_t R, int64_t dh) { return dtype == FF_F32 || R <= 128 ? 0 : dh == 256 ? 4 : 8; }
 
 static AttPlan attention_plan(const ff_cache_attention_t* a) {
@@ -673,9 +678,9 @@ static int launch_join_groups(const ff_cache_attention_t* a, const AttPlan& p) {
 }
 template <int DT, int DH>
 static int launch_join(const ff_cache_attention_t* a, const AttPlan& p) {
-    // (6 832 rows of 30 slots: 11 us a group a row, 8 us four)
+    // (6 832 rows of 32 slots: 8.2 us with four groups a row, 8.3 us with one)
     if (a->cache.B * a->cache.kv_heads * p.R >= 1024) return launch_join_groups<DT, DH, DH / 4, DH == 256 ? 2 : 4>(a, p);
-    // (28 rows: 256 slots 8.4 us with the rows whole, 3.5 us in pieces; 33 slots 3.2 and 4.0)
+    // (28 rows: 256 slots 12.3 us with the rows whole, 7.1 us in pieces; 33 slots 3.9 and 4.5; 56 rows of 258 slots 7.0 and 6.2)
     return p.slots > 64 ? launch_join_groups<DT, DH, 8, 32>(a, p) : launch_join_groups<DT, DH, DH / 4, kJoinThreads / (DH / 4)>(a, p);
 }
 template <int DT>

@@ -8,9 +8,10 @@
 // wants, so the weights never leave the registers; V^T comes out of shared memory by the transposing reads (ds_read_b64_tr_b16:
 // 16 lanes that point at 4 rows of 16 channels get one channel of 4 rows each).  At 32 rows a wave a product is fed by one
 // read of 16 bytes a lane, which shared memory keeps up with; what a step costs is its products, its softmax (an exponential a score, at
-// a quarter of the rate) and the barrier, which the two waves of a SIMD overlap only in part.  4 sequences of up to 13 474 keys in bf16, 61
-// new tokens, 28 / 4 heads of 128: 52 us, 5 to 8 us of that the join and about 14 us the way to the first keys and out (lengths, pages,
-// Q, partial rows).  A higher priority for one wave of each SIMD changed nothing (50 to 56 us with and without).
+// a quarter of the rate) and the barrier, which the two waves of a SIMD overlap only in part.  28 / 4 heads of 128, 4 sequences, 61 new
+// tokens in bf16, 1 to 52 steps of 64 keys a workgroup: 15 us (the way to the first keys and out: lengths, pages, Q, partial rows) and 2.35 us
+// a step, of which the products are 1.5 at the rate of a large one; the join takes 8.  Over up to 13 474 keys: 47 us + 8.  A higher priority
+// for one wave of each SIMD changed nothing (50 to 56 us with and without).
 #include <atomic>
 
 #include "ff_attend.h"
@@ -295,7 +296,7 @@ __global__ __launch_bounds__(64 * NW, DH == 256 ? 1 : 2) void k_cache_attention_
             };
             // values are read while the weights that meet them are made, and the first half's products run under the second half's
             // softmax; the barriers keep the compiler from undoing that.  (256 channels: the outputs and Q leave no registers for it - 64 new
-            // tokens of 28 / 4 heads over 8 x 20 000 keys 920 us spilling, 709 us with the values read behind the weights)
+            // tokens of 28 / 4 heads over 8 x 20 000 keys 920 us spilling, 700 us with the values read behind the weights)
             score();
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (kShared) load_values(0);

@@ -11,7 +11,7 @@ constexpr int kStoreSame = 0;   // template value: the cache holds T itself
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-// 2^(byte - 127); byte 0 stands for a block of zeros, 255 for a block of NaN
+// 2^(byte - 127); 255 stands for a block of NaN, 0 for a row that was never written (its codes are zeros)
 __device__ inline float block_scale(uint32_t byte) { return __uint_as_float(byte == 255u ? 0x7fc00000u : byte << 23); }
 
 // bytes of one row of `dh` channels

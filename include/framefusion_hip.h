@@ -403,7 +403,8 @@ int ff_rotary_tables(const int64_t* positions, int64_t n, const double* inv_freq
 int ff_rotary_apply(const ff_rotary_t* args);
 
 /* The cache: keys and values [n_pages, kv_heads, page_size, dh] in T (store = the dtype code) or as codes with one scale byte
- * for each 32 channels, [n_pages, kv_heads, page_size, dh / 32]: value = code * 2^(byte - 127), byte 0 = the block is zero, 255 = it is NaN.
+ * for each 32 channels, [n_pages, kv_heads, page_size, dh / 32]: value = code * 2^(byte - 127), 255 = the block is NaN.  Byte 0 is that of
+ * rows that nothing was written to, whose codes are zeros (ff_cache_write gives 27 to 254, or 255).
  * FF_STORE_E4M3: one byte a channel.  FF_STORE_E2M1: half a byte, the even channel in the low half.  Position p of sequence b
  * is row p % page_size of page table[b * table_width + p / page_size]; a position past the table or with an entry outside
  * [0, n_pages) has no place: it is not written, reads as zeros and is not attended to.  start[b] = tokens before the n that
@@ -441,7 +442,8 @@ int ff_cache_keep(const ff_cache_t* cache, const int32_t* accepted, int64_t m, f
 /* ff_cache_attention: out_i = sum_j softmax_j(scale q_i . k_j) v_j for the n new tokens of each sequence, whose keys and values
  *   lie in the cache behind its start[b] earlier ones.  Token i sees every earlier token, and new token j where
  *   mask[b * mask_batch + i * n + j] != 0 (mask = NULL: j <= i).  What it does not see contributes nothing, whatever is stored
- *   there; a token that sees nothing gets zeros.  |scale| <= 1e30.  Scores, statistics and sums in fp32; the probabilities are rounded to T before
+ *   there; a token that sees nothing gets zeros.  An infinity among the values of earlier tokens comes out as an infinity, or as NaN where
+ *   its weight is below T's smallest number.  n * H <= 983 024, B <= 65 535.  |scale| <= 1e30.  Scores, statistics and sums in fp32; the probabilities are rounded to T before
  *   they meet the values.  ws: ff_cache_attention_workspace_bytes(args) bytes (may be 0), not initialised, dead when the call's
  *   work is done. */
 typedef struct ff_cache_attention {
