@@ -88,3 +88,24 @@ def test_zeros_without_memory():
     cos = torch.ones(1, 5, 64, device=DEV).bfloat16()
     for got, x in zip(ffa.apply_rotary(q, zero(k), cos, zero(cos)), (q, torch.zeros_like(k))):
         assert torch.equal(got, x)
+
+
+# ---- infinities among earlier tokens' values
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [1, 9, 64])
+def test_an_infinite_value_of_an_earlier_token(dtype, n):
+    """All new tokens see it: infinity in its channel, NaN where two of other signs meet, nothing elsewhere.  (Scores of deviation
+    1/4: no weight is small beside another.)"""
+    gen = torch.Generator(device=DEV).manual_seed(n)
+    cache = ffa.new_cache(8, 32, 2, 64, dtype, None, device=DEV)
+    table, start = torch.arange(8, dtype=torch.int32, device=DEV)[None], torch.tensor([150], dtype=torch.int32, device=DEV)
+    k, v = (torch.randn(1, 2, 150 + n, 64, generator=gen, device=DEV).to(dtype) for _ in range(2))
+    k[:, :, [7, 140]] = 0                                                   # score 0: their weight is not small beside any other's
+    v[:, :, 7, 3], v[:, :, 140, 9] = float("inf"), float("-inf")
+    v[:, :, 7, 20], v[:, :, 140, 20] = float("inf"), float("-inf")
+    ffa.cache_write(cache, k, v, table, torch.zeros_like(start))
+    q = (torch.randn(1, 6, n, 64, generator=gen, device=DEV) * 0.25).to(dtype)
+    got = ffa.cache_attention(q, cache, table, start)[0]
+    assert (got[..., 3] == float("inf")).all() and (got[..., 9] == float("-inf")).all() and torch.isnan(got[..., 20]).all()
+    rest = [i for i in range(64) if i not in (3, 9, 20)]
+    assert torch.isfinite(got[..., rest]).all()

@@ -47,3 +47,44 @@ def test_positions_of_other_integer_types():
         got, want = (model.model(inputs_embeds=x, past_key_values=c, use_cache=True, position_ids=positions("qwen2", [310, 311]).to(t)).last_hidden_state
                      for c, t in zip(caches, (torch.int32, torch.int64)))
         assert torch.equal(got, want)
+
+
+def test_the_full_qwen2_vl_model_counts_on_from_the_unreduced_prompt():
+    """Its own positions are (tokens seen) + (the prompt's M-RoPE offset): they need the unreduced count."""
+    from transformers import Qwen2VLConfig, Qwen2VLForConditionalGeneration
+    from transformers.cache_utils import DynamicCache
+    from framefusion_amd.models.qwen2_vl import register_hf_qwen2_vl
+    from tests.test_gpu_reduced_cache import close
+    torch.manual_seed(0)
+    VID = 151
+    cfg = Qwen2VLConfig(
+        text_config=dict(vocab_size=160, hidden_size=256, intermediate_size=512, num_hidden_layers=4, num_attention_heads=8, num_key_value_heads=2,
+                         max_position_embeddings=4096, bos_token_id=None, eos_token_id=None,
+                         rope_parameters={"rope_type": "default", "rope_theta": 1e6, "mrope_section": [4, 6, 6]}),
+        vision_config=dict(depth=1, embed_dim=32, hidden_size=256, num_heads=2, mlp_ratio=2, in_channels=3, patch_size=14, spatial_merge_size=2, temporal_patch_size=2),
+        image_token_id=150, video_token_id=VID, vision_start_token_id=152, vision_end_token_id=153)
+    cfg._attn_implementation = "sdpa"
+    model = Qwen2VLForConditionalGeneration(cfg).to(DEV).eval()
+    register_hf_qwen2_vl()
+    ffa.apply_framefusion(model, cost=0.3, similarity_lower_bound=0.5, ratio_lower_bound=0.1)
+    T, H, W = 12, 8, 12
+    n = T * H * W // 4
+    ids = torch.tensor([[1, 2, 3, 4, 152] + [VID] * n + [153, 5, 6, 7, 8, 9, 10]], device=DEV)
+    frame = torch.randn(H * W, 3 * 2 * 14 * 14)
+    frames = [frame]
+    for t in range(1, T):
+        frames.append(torch.randn_like(frame) if t in (5, 9) else frames[-1] + 0.05 * torch.randn_like(frame))
+    video = dict(pixel_values_videos=torch.cat(frames).to(DEV), video_grid_thw=torch.tensor([[T, H, W]], device=DEV), mm_token_type_ids=(ids == VID).int() * 2)
+    left, told = (ffa.ReducedCache(4, 2, 32, 512, dtype=torch.float32, device=DEV) for _ in range(2))
+    old = DynamicCache(config=cfg.text_config)
+    token = torch.tensor([[11]], device=DEV)
+    with torch.no_grad():
+        for cache in (left, told, old):
+            model.model(input_ids=ids, past_key_values=cache, use_cache=True, **video)
+        L, delta = ids.shape[1], int(model.model.rope_deltas)
+        assert left.seen == L and left.lengths[0] < L and delta != 0
+        for i in range(2):
+            at = torch.full((3, 1, 1), L + i + delta, device=DEV)
+            got = model.model(input_ids=token, past_key_values=left, use_cache=True).last_hidden_state
+            assert torch.equal(got, model.model(input_ids=token, past_key_values=told, use_cache=True, position_ids=at).last_hidden_state)
+            close(got, model.model(input_ids=token, past_key_values=old, use_cache=True, position_ids=at).last_hidden_state)
